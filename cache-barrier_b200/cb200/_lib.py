@@ -24,6 +24,7 @@ CB_ERR_CUDA = 7
 CB_ERR_DEVICE_TIMEOUT = 8
 CB_ERR_UNSUPPORTED = 9
 CB_ERR_TOO_LARGE = 10
+CB_ERR_DEVICE_INDEX = 11
 
 # dtype codes
 CB_DTYPE_F16 = 0
@@ -32,12 +33,20 @@ CB_DTYPE_F32 = 2
 CB_DTYPE_I8 = 3
 CB_DTYPE_U8 = 4
 CB_DTYPE_I32 = 5
+CB_DTYPE_E4M3 = 6
 
 # ops
 CB_OP_W8A8 = 0
 CB_OP_W4A16 = 1
 CB_OP_W4A4 = 2
 CB_OP_NVFP4 = 3
+CB_OP_FP8_BLOCK = 4
+CB_OP_PAGED_ATTENTION = 5
+
+# output forms of the residual RMSNorm
+CB_NORM_INT8 = 0
+CB_NORM_FP8 = 1
+CB_NORM_FP8_BLOCK = 2
 
 # fp8 activation quantization modes
 CB_FP8_PER_TOKEN = 0
@@ -96,6 +105,16 @@ SIGNATURES = {
     "cb_repack_w8_kmajor": (_int, [_vp, _vp, _i64, _i64, _i64, _vp]),
     "cb_rmsnorm_quant_i8": (_int, [_vp, _int, _vp, _int, ctypes.c_float, _i64, _i64, _i64, _vp, _i64, _vp, _vp,
                                    _i64, _vp]),
+    "cb_add_rmsnorm_quant": (_int, [_vp, _vp, _int, _vp, _int, ctypes.c_float, _i64, _i64, _i64, _i64, _int, _vp, _i64,
+                                    _vp, _i64, _vp, _i64, _vp]),
+    "cb_quant_act_fp8_block": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "cb_fp8_block_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "cb_fp8_block_gemm_dynamic": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _int, _vp, _int, _i64, _i64,
+                                         _i64, _i64, _vp, _vp, _sz, _vp]),
+    "cb_paged_kv_append": (_int, [_vp, _vp, _int, _vp, _vp, _int, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp,
+                                  _vp, _vp]),
+    "cb_paged_decode_attention": (_int, [_vp, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _i64,
+                                         _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _sz, _vp]),
     "cb_symm_bytes": (_sz, [_int, _i64]),
     "cb_symm_alloc": (_int, [_sz, ctypes.POINTER(_vp)]),
     "cb_symm_free": (_int, [_vp]),

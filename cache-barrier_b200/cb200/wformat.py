@@ -14,7 +14,8 @@ once, offline) and stores the kernel-ready bytes with their scales:
                          "crc32", and per kind "batch", "K", "N", "group_size"}]}
 
 ``kind`` is ``w4_native`` (uint8 bytes of the native layout), ``w8_kmajor``
-(int8 [B, N, K]) or ``scales`` / ``raw`` (any numpy dtype). ``load`` checks
+(int8 [B, N, K]), ``fp8_block`` (e4m3 bytes [B, N, K], K-major, with one fp32 scale per
+128 x 128 block) or ``scales`` / ``raw`` (any numpy dtype). ``load`` checks
 every CRC and returns numpy arrays, or torch tensors on ``device``.
 """
 
@@ -100,6 +101,46 @@ class PackedInt8:
     scales: np.ndarray  # fp32 [B, N]
 
 
+@dataclass
+class PackedFp8Block:
+    w_nk: np.ndarray  # e4m3 bytes: uint8 [B, N, K] (float8_e4m3fn on a device)
+    scales: np.ndarray  # fp32 [B, ceil(N / 128), ceil(K / 128)]
+
+
+def _e4m3_bytes(v: np.ndarray) -> np.ndarray:
+    """fp32 -> e4m3 bytes, to nearest even, saturated at 448 (NaN stays NaN)."""
+    v = np.asarray(v, dtype=np.float32)
+    mag = np.where(np.isnan(v), np.float32(0.0), np.minimum(np.abs(v), np.float32(448.0)))
+    exp = np.maximum(np.frexp(mag)[1] - 1, -6)  # exponent of the value; subnormals share that of 2^-6
+    steps = np.rint(np.ldexp(mag.astype(np.float64), 3 - exp)).astype(np.int64)  # eighths of 2^exp: 8..16, below 8 subnormal
+    code = np.where(mag == 0, 0, (exp + 6) * 8 + steps)  # a carry to 16 is the next exponent's 8
+    code = np.where(np.isnan(v), 0x7F, code)
+    return (code | (np.signbit(v).astype(np.int64) << 7)).astype(np.uint8)
+
+
+def quantize_fp8_block(w) -> PackedFp8Block:
+    """A floating-point weight [N, K] or [B, N, K] (numpy or torch) as e4m3 with one
+    scale per 128 x 128 block, max(amax / 448, 1 / (448 * 512)): the operands of
+    ``ops.fp8_block_gemm``. Blocks at the ends of N and K may be partial."""
+    try:
+        import torch
+
+        if isinstance(w, torch.Tensor):
+            w = w.detach().float().cpu().numpy()
+    except ImportError:  # pragma: no cover
+        pass
+    w = np.asarray(w, dtype=np.float32)
+    w = w[None] if w.ndim == 2 else w
+    B, N, K = w.shape
+    nb, kb = -(-N // 128), -(-K // 128)
+    full = np.zeros((B, nb * 128, kb * 128), dtype=np.float32)
+    full[:, :N, :K] = w
+    t = full.reshape(B, nb, 128, kb, 128)
+    scales = np.maximum(np.abs(t).max(axis=(2, 4)) / np.float32(448.0), np.float32(1.0 / (448.0 * 512.0)))
+    q = _e4m3_bytes(t / scales[:, :, None, :, None]).reshape(full.shape)[:, :N, :K]
+    return PackedFp8Block(np.ascontiguousarray(q), scales)
+
+
 def pack_int4(src, layout: int, K: int, N: int, scales, group_size: int) -> PackedInt4:
     """``scales`` may be a numpy array or a torch tensor (bf16 kept as bf16)."""
     src = _to_numpy(src)
@@ -144,13 +185,17 @@ def _entries(tensors: dict) -> list[_Entry]:
             B, N, K = t.w_nk.shape
             out.append(_Entry(name, "w8_kmajor", t.w_nk, {"batch": B, "K": K, "N": N}))
             out.append(_entry(name + ".scales", "scales", t.scales, {}))
+        elif isinstance(t, PackedFp8Block):
+            B, N, K = t.w_nk.shape
+            out.append(_Entry(name, "fp8_block", t.w_nk, {"batch": B, "K": K, "N": N}))
+            out.append(_entry(name + ".scales", "scales", t.scales, {}))
         else:
             out.append(_entry(name, "raw", t, {}))
     return out
 
 
 def save(path: str, tensors: dict, meta: dict | None = None) -> None:
-    """Writes packed weights (PackedInt4 / PackedInt8) and raw arrays. torch tensors
+    """Writes packed weights (PackedInt4 / PackedInt8 / PackedFp8Block) and raw arrays. torch tensors
     are accepted and stored by dtype name (bfloat16 as its 16-bit pattern)."""
     ents = _entries({k: _to_numpy(v) for k, v in tensors.items()})
     descs, blobs, offset = [], [], 0
@@ -190,11 +235,14 @@ def _to_numpy(v):
         return PackedInt4(_to_numpy(v.native), _to_numpy(v.scales), v.batch, v.K, v.N, v.group_size)
     if isinstance(v, PackedInt8):
         return PackedInt8(_to_numpy(v.w_nk), _to_numpy(v.scales))
+    if isinstance(v, PackedFp8Block):
+        bits = v.w_nk if isinstance(v.w_nk, np.ndarray) else v.w_nk.view(torch.uint8)
+        return PackedFp8Block(_to_numpy(bits), _to_numpy(v.scales))
     return v
 
 
 def load(path: str, device=None) -> dict:
-    """Reads a file written by ``save``. Returns {name: PackedInt4 | PackedInt8 | array};
+    """Reads a file written by ``save``. Returns {name: PackedInt4 | PackedInt8 | PackedFp8Block | array};
     with ``device`` the arrays are torch tensors on it (bf16 restored)."""
     with open(path, "rb") as f:
         data = f.read()
@@ -223,6 +271,13 @@ def load(path: str, device=None) -> dict:
                                    d["N"], d["group_size"])
         elif d["kind"] == "w8_kmajor":
             out[name] = PackedInt8(_dev(a, "int8", device), _dev(sc[1], sc[0]["dtype"], device))
+        elif d["kind"] == "fp8_block":
+            w = _dev(a, "uint8", device)
+            if device is not None:
+                import torch
+
+                w = w.view(torch.float8_e4m3fn)
+            out[name] = PackedFp8Block(w, _dev(sc[1], sc[0]["dtype"], device))
         else:
             out[name] = _dev(a, d["dtype"], device)
     return out

@@ -9,6 +9,7 @@
 
 #include "cb200.h"
 #include "cb_internal.h"
+#include "cb_ptx.cuh"
 
 namespace cb {
 
@@ -254,7 +255,7 @@ int read_and_clear_status(void* scratch, int* device_status, cudaStream_t s) {
     // them with the status word so the next call starts from zero.
     if (cudaMemsetAsync(scratch, 0, kWsHeader + kWsCounters, s) != cudaSuccess) return CB_ERR_CUDA;
     if (cudaStreamSynchronize(s) != cudaSuccess) return CB_ERR_CUDA;
-    return CB_ERR_DEVICE_TIMEOUT;
+    return (host & CB_DEVERR_TIMEOUT) ? CB_ERR_DEVICE_TIMEOUT : CB_ERR_DEVICE_INDEX;
   }
   return CB_OK;
 }
@@ -289,6 +290,8 @@ const char* cb_status_str(int status) {
       return "unsupported device or layout";
     case CB_ERR_TOO_LARGE:
       return "size beyond the supported maximum";
+    case CB_ERR_DEVICE_INDEX:
+      return "cache slot, page index or length outside the cache";
     default:
       return "unknown status";
   }
@@ -307,6 +310,10 @@ size_t cb_workspace_bytes(int op, int64_t batch, int64_t M, int64_t N, int64_t K
       return w4a16_workspace_bytes(batch, M, N, K);
     case CB_OP_NVFP4:
       return nvfp4_workspace_bytes(M);
+    case CB_OP_FP8_BLOCK:
+      return fp8_block_workspace_bytes(M);
+    case CB_OP_PAGED_ATTENTION:
+      return paged_attention_workspace_bytes(M, N, K);
     case CB_OP_W4A4: {
       // the int8 GEMM scratch, then unpacked A [M, K] and B [N, K] (8-bit).
       const size_t a = align_up(static_cast<size_t>(M) * K, 256);

@@ -190,4 +190,11 @@ int launch_nvfp4_quant(const void* x, int x_dtype, int64_t rows, int64_t K, int6
                        uint8_t* q, int64_t q_sm, uint8_t* sf, cudaStream_t stream);
 size_t nvfp4_workspace_bytes(int64_t M);
 
+// e4m3 with one scale per 128 elements of a row (add_rmsnorm_quant.cu).
+int launch_quant_fp8_block(const void* a, int a_dtype, int64_t batch, int64_t M, int64_t K, int64_t a_sb, int64_t a_sm,
+                           uint8_t* q, int64_t q_sb, int64_t q_sm, float* scale, int64_t s_sb, int64_t s_sm,
+                           cudaStream_t stream);
+size_t fp8_block_workspace_bytes(int64_t M);
+size_t paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D);
+
 }  // namespace cb

@@ -21,6 +21,8 @@ constexpr unsigned long long kWaitLimitNs = 1000ull * 1000ull * 1000ull;
 
 // Device-side status bits written to the status word in the workspace.
 constexpr int CB_DEVERR_TIMEOUT = 1;
+// A cache slot, page index or length outside the cache: the access was skipped.
+constexpr int CB_DEVERR_BAD_INDEX = 2;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -1,0 +1,691 @@
+// Attention of one new token per sequence over a paged key-value cache:
+//   z_l = scale * (q . k_l),  out = sum_l softmax(z)_l v_l,  lse = log sum_l exp(z_l)
+// over the seq_lens[b] tokens that block_table[b] maps to cache pages; query heads
+// share key-value heads in groups of G. bf16 / f16 queries; the cache has the
+// queries' type or is e4m3 with one scale per head.
+//
+// Bound: HBM on the cache (2 * L * heads * D elements read once; 2G flops per
+// byte of a 16-bit cache).
+//
+// One pass with a running maximum and sum. All (sequence, kv head, head block)
+// items are cut into tiles of kTile tokens, laid end to end, and the tiles are
+// dealt to the CTAs in equal contiguous ranges, so ragged lengths load every SM
+// alike. An item inside one CTA's range is finished there; a cut item's parts
+// (max, sum, unnormalised output per head) go to the workspace and the CTA whose
+// atomic completes the item's count joins them in CTA order: no CTA waits, and
+// the bits do not depend on who joins.
+//
+// A CTA is four warps, and each warp is a worker of its own: it takes 16 of a
+// tile's tokens and keeps its own running maximum, sum and output, so the loop
+// has no barrier; the warps are joined at the item's end. Keys and values go from
+// global memory straight into matrix-instruction fragments:
+//   S^T[token, head] = K Q^T   m16n8k16, rows = tokens, columns = up to 8 heads
+//   O^T[d, head]    += V^T P^T m16n8k16, rows = d, k = tokens
+// The order of d inside a k-step and of the output rows is free, so a lane's
+// 16-byte loads of K (token g, d 8t..8t+7) and V (tokens 2t, 2t+1, 2t+8, 2t+9,
+// d 8g..8g+7) are the fragments after byte permutes, with no shared memory.
+// P^T is the transpose of the S^T accumulator: one movmatrix per 8 tokens. Heads
+// are the narrow side (n = 8): a group of 5 to 8 wastes little and one wasted
+// column costs no bandwidth. mma.sync is enough here: at 8 heads the products
+// need a few percent of its rate at full cache bandwidth, and tcgen05 would need
+// the tiles staged in shared memory first.
+//
+// e4m3 caches run in f16 (every e4m3 value is an f16 value): the query row is
+// scaled by a power of two into f16's range, and that factor and the head's key
+// scale return in the fp32 score.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "cb_internal.h"
+#include "cb_ptx.cuh"
+
+namespace cb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 16 * kWarps;  // tokens per tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct AttnParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int* table;
+  const int* lens;
+  const float* k_scale;  // optional, per kv head
+  const float* v_scale;
+  void* out;
+  float* lse;  // optional
+  float scale;
+  int B, heads, G, blocks;  // kv heads, queries per kv head, head blocks (of 8 * NT queries) per kv head
+  int num_pages, page, page_shift, max_pages;  // page_shift: log2(page) or -1
+  long long q_sb, q_sh, o_sb, o_sh, lse_sb, table_sb;
+  long long k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;  // in bytes
+  int* status;
+  int* counters;
+  float* partials;
+};
+
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// 16-bit arithmetic type of the products: bf16, or f16 (f16 queries, e4m3 caches).
+template <bool BF16>
+struct Math;
+template <>
+struct Math<true> {
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+template <>
+struct Math<false> {
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+
+// Two e4m3 values (exact) as f16x2.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+__device__ __forceinline__ float q_val(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float q_val(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void put(__half* o, float v) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* o, float v) { *o = __float2bfloat16_rn(v); }
+
+// Inclusive sum over the CTA's threads; *total receives the whole sum.
+__device__ __forceinline__ long long block_scan(long long v, long long* sh, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = v;
+  __syncthreads();
+  long long sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) v += sum;
+    sum += sh[w];
+  }
+  *total = sum;
+  return v;
+}
+
+template <typename QT, bool FP8, int D, int NT>
+struct Shape {
+  static constexpr bool kBf16 = std::is_same<QT, __nv_bfloat16>::value && !FP8;
+  // Probabilities relative to the running maximum carry a factor 2^kShift, which
+  // the division by their sum takes out: f16 then keeps them normal down to 2^-29
+  // instead of 2^-14 (a long context's typical weight). bf16 has fp32's range.
+  static constexpr float kShift = kBf16 ? 0.0f : 15.0f;
+  static constexpr int kElem = FP8 ? 1 : 2;
+  static constexpr int kHeads = 8 * NT;          // query heads of a head block
+  static constexpr int kKC = D * kElem / 64;     // 16-byte chunks of K per lane and token (four lanes share a row)
+  static constexpr int kVLane = D * kElem / 8;   // bytes of V per lane and token (eight lanes share a row)
+  static constexpr int kVV = kVLane >= 16 ? 16 : 8;  // bytes of one load
+  static constexpr int kVC = kVLane / kVV;
+  static constexpr int kKSteps = D / 16;
+  // part of a cut item: max and sum per head, output per head and d
+  static constexpr int kPart = kHeads * 2 + kHeads * D;
+  static constexpr size_t kSmem = sizeof(float) * kWarps * kPart + sizeof(uint2) * kKSteps * NT * 32;
+};
+
+template <typename QT, bool FP8, int D, int NT, bool PAGE16>
+__global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
+  using S = Shape<QT, FP8, D, NT>;
+  using M = Math<S::kBf16>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  float* const sh_part = reinterpret_cast<float*>(smem_raw);  // [warp][kPart]
+  uint2* const sh_q = reinterpret_cast<uint2*>(sh_part + kWarps * S::kPart);  // query fragments [k-step][NT][lane]
+  __shared__ long long sh_scan[kWarps];
+  __shared__ long long sh_found[2];
+  __shared__ float sh_qexp[S::kHeads];
+  __shared__ int sh_last;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+
+  const long long cap = static_cast<long long>(p.max_pages) * p.page;
+  bool bad = false;
+  auto length = [&](int b) {
+    const int n = p.lens[b];
+    if (n < 0 || n > cap) bad = true;
+    return n < 0 ? 0 : n > cap ? static_cast<int>(cap) : n;
+  };
+  const int per_b = p.heads * p.blocks;  // items per sequence
+  // Sequences without tokens: zeros and a log sum of -inf.
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    if (length(b) > 0) continue;
+    for (int i = tid; i < p.heads * p.G * D; i += kThreads) {
+      const int h = i / D;
+      put(static_cast<QT*>(p.out) + b * p.o_sb + h * p.o_sh + (i - h * D), 0.0f);
+    }
+    if (p.lse)
+      for (int h = tid; h < p.heads * p.G; h += kThreads) p.lse[b * p.lse_sb + h] = -INFINITY;
+  }
+  // This CTA's tiles [t0, t1) of the T tiles, and the sequence that holds t0.
+  long long T = 0;
+  for (int base = 0; base < p.B; base += kThreads) {
+    const int b = base + tid;
+    const long long n = b < p.B ? static_cast<long long>((length(b) + kTile - 1) / kTile) * per_b : 0;
+    long long sum;
+    block_scan(n, sh_scan, &sum);
+    T += sum;
+  }
+  if (bad && p.status) atomicOr(p.status, CB_DEVERR_BAD_INDEX);
+  // no more CTAs than tiles take part, so every one between an item's first and last holds a part of it
+  const int grid = T < static_cast<long long>(gridDim.x) ? static_cast<int>(T) : static_cast<int>(gridDim.x);
+  const int cta = static_cast<int>(blockIdx.x);
+  if (cta >= grid) return;
+  const long long t0 = cta * T / grid, t1 = (cta + 1) * T / grid;
+  long long before = 0;
+  for (int base = 0; base < p.B; base += kThreads) {
+    const int b = base + tid;
+    const long long n = b < p.B ? static_cast<long long>((length(b) + kTile - 1) / kTile) * per_b : 0;
+    long long sum;
+    const long long incl = block_scan(n, sh_scan, &sum) + before;
+    if (t0 >= incl - n && t0 < incl) {
+      sh_found[0] = b;
+      sh_found[1] = incl - n;
+    }
+    before += sum;
+    if (t0 < before) break;  // uniform
+  }
+  __syncthreads();
+  int b = static_cast<int>(sh_found[0]);
+  int len = length(b);
+  int tiles = (len + kTile - 1) / kTile;
+  int item = static_cast<int>((t0 - sh_found[1]) / tiles);         // item within the sequence
+  int tile = static_cast<int>(t0 - sh_found[1] - static_cast<long long>(item) * tiles);  // tile within the item
+  long long at = t0;
+
+  while (at < t1) {
+    const int head = item / p.blocks, blk = item - head * p.blocks;
+    const int q0 = blk * S::kHeads;                                   // first query of the block, within its group
+    const int nq = p.G - q0 < S::kHeads ? p.G - q0 : S::kHeads;       // queries of the block
+    const int tile_end = tiles - tile < t1 - at ? tiles : tile + static_cast<int>(t1 - at);
+    const long long item_first = at - tile;  // global index of the item's first tile
+    const QT* qrow = static_cast<const QT*>(p.q) + b * p.q_sb + static_cast<long long>(head * p.G + q0) * p.q_sh;
+
+    // ---- query fragments ----
+    __syncthreads();  // the previous item is done with the shared memory
+    if constexpr (FP8) {
+      // power of two that brings each query row's largest value to [1, 2)
+      for (int r = warp; r < S::kHeads; r += kWarps) {
+        float m = 0.0f;
+        if (r < nq)
+          for (int d = lane; d < D; d += 32) m = fmaxf(m, fabsf(q_val(qrow + r * p.q_sh + d)));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        int e = 0;
+        if (m > 0.0f && m < INFINITY) e = ilogbf(m);
+        if (e < -100) e = -100;  // rows below 2^-100 keep a factor that fp32 holds
+        if (lane == 0) sh_qexp[r] = ldexpf(1.0f, e);
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < S::kKSteps * NT * 32; i += kThreads) {
+      const int l = i & 31, r = (i >> 5) % NT * 8 + (l >> 2), ks = (i >> 5) / NT;
+      // d of the k-step's four elements in lane t: the order of K's 16-byte chunks
+      const int d = FP8 ? (ks >> 2) * 64 + (l & 3) * 16 + (ks & 3) * 4 : (ks >> 1) * 32 + (l & 3) * 8 + (ks & 1) * 4;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < nq) {
+        const float f = FP8 ? 1.0f / sh_qexp[r] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = q_val(qrow + r * p.q_sh + d + j) * f;
+      }
+      sh_q[i] = make_uint2(M::pack(v[0], v[1]), M::pack(v[2], v[3]));
+    }
+    __syncthreads();
+    float zs[NT][2];  // score factor of this lane's two heads
+    const float ks_head = FP8 && p.k_scale ? p.k_scale[head] : 1.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        zs[n][j] = p.scale * kLog2e;
+        if constexpr (FP8) zs[n][j] = p.scale * ks_head * sh_qexp[n * 8 + 2 * t + j] * kLog2e;
+      }
+
+    float o[S::kKSteps][NT][4];
+    float m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int i = 0; i < S::kKSteps; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][n][j] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) m_run[n][j] = -INFINITY, l_run[n][j] = 0.0f;
+
+    const int* trow = p.table + b * p.table_sb;
+    const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + head * p.k_sh;
+    const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + head * p.v_sh;
+    auto page_of = [&](int tok) { return p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page; };
+    // Cache page of a token; -1 past the length or where the table is wrong.
+    auto lookup = [&](int tok) {
+      if (tok >= len) return -1;
+      const int pg = trow[page_of(tok)];
+      if (static_cast<unsigned>(pg) >= static_cast<unsigned>(p.num_pages)) {
+        if (p.status) atomicOr(p.status, CB_DEVERR_BAD_INDEX);
+        return -1;
+      }
+      return pg;
+    };
+
+    for (int tl = tile; tl < tile_end; ++tl) {
+      const int tok0 = tl * kTile + warp * 16;
+      if (tok0 >= len) break;  // the item's last tile: no token for this warp
+      // page of this lane's token (lane & 15); with PAGE16 all 16 share one page
+      const int my_pg = lookup(PAGE16 ? tok0 : tok0 + (lane & 15));
+      uint4 kr[2][S::kKC];
+      uint4 vr[4][S::kVC];
+      bool k_ok[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int rel = g + 8 * r, tok = tok0 + rel;
+        const int pg = PAGE16 ? my_pg : __shfl_sync(0xffffffffu, my_pg, rel);
+        k_ok[r] = tok < len && pg >= 0;
+        const uint8_t* row = kbase + pg * p.k_sp + static_cast<long long>(tok - page_of(tok) * p.page) * p.k_ss + t * 16;
+#pragma unroll
+        for (int c = 0; c < S::kKC; ++c) kr[r][c] = k_ok[r] ? ldg16(row + c * 64) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int rel = 2 * t + (r & 1) + 8 * (r >> 1), tok = tok0 + rel;
+        const int pg = PAGE16 ? my_pg : __shfl_sync(0xffffffffu, my_pg, rel);
+        const bool ok = tok < len && pg >= 0;
+        const uint8_t* row =
+            vbase + pg * p.v_sp + static_cast<long long>(tok - page_of(tok) * p.page) * p.v_ss + g * S::kVV;
+#pragma unroll
+        for (int c = 0; c < S::kVC; ++c) {
+          if constexpr (S::kVV == 16) {
+            vr[r][c] = ok ? ldg16(row + c * 128) : make_uint4(0, 0, 0, 0);
+          } else {
+            const uint2 two = ok ? ldg8(row + c * 64) : make_uint2(0, 0);
+            vr[r][c] = make_uint4(two.x, two.y, 0, 0);
+          }
+        }
+      }
+      // ---- scores ----
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < S::kKC; ++c) {
+        const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&kr[0][c]);
+        const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&kr[1][c]);
+#pragma unroll
+        for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (FP8) {
+            a0 = e4m3x2_f16x2(w0[i]), a1 = e4m3x2_f16x2(w1[i]);
+            a2 = e4m3x2_f16x2(w0[i] >> 16), a3 = e4m3x2_f16x2(w1[i] >> 16);
+          } else {
+            a0 = w0[2 * i], a1 = w1[2 * i], a2 = w0[2 * i + 1], a3 = w1[2 * i + 1];
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 bq = sh_q[((c * (FP8 ? 4 : 2) + i) * NT + n) * 32 + lane];
+            M::mma(s[n], a0, a1, a2, a3, bq.x, bq.y);
+          }
+        }
+      }
+      // ---- running maximum and sum ----
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float x[4], mx[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = k_ok[j >> 1] ? s[n][j] * zs[n][j & 1] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mx[j] = fmaxf(x[j], x[2 + j]);
+#pragma unroll
+          for (int sft = 4; sft < 32; sft <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], sft));
+          mx[j] = fmaxf(mx[j], m_run[n][j]);
+        }
+        float al[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float ref = mx[j] == -INFINITY ? 0.0f : mx[j];
+          al[j] = exp2_approx(m_run[n][j] - ref);
+          m_run[n][j] = mx[j];
+          x[j] = exp2_approx(x[j] - ref + S::kShift);
+          x[2 + j] = exp2_approx(x[2 + j] - ref + S::kShift);
+          l_run[n][j] = l_run[n][j] * al[j] + (x[j] + x[2 + j]);
+        }
+        if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < S::kKSteps; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][n][j] *= al[j & 1];
+        }
+        pb[n][0] = movmatrix_trans(M::pack(x[0], x[1]));
+        pb[n][1] = movmatrix_trans(M::pack(x[2], x[3]));
+      }
+      // ---- output ----
+#pragma unroll
+      for (int c = 0; c < S::kVC; ++c) {
+        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vr[0][c]);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vr[1][c]);
+        const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vr[2][c]);
+        const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vr[3][c]);
+#pragma unroll
+        for (int w = 0; w < S::kVV / 4; ++w) {
+          if constexpr (FP8) {
+#pragma unroll
+            for (int hl = 0; hl < 2; ++hl) {
+              const uint32_t lo = __byte_perm(v0[w], v1[w], hl ? 0x7362 : 0x5140);
+              const uint32_t hi = __byte_perm(v2[w], v3[w], hl ? 0x7362 : 0x5140);
+              const uint32_t a0 = e4m3x2_f16x2(lo), a1 = e4m3x2_f16x2(lo >> 16);
+              const uint32_t a2 = e4m3x2_f16x2(hi), a3 = e4m3x2_f16x2(hi >> 16);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) M::mma(o[(c * (S::kVV / 4) + w) * 2 + hl][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+            }
+          } else {
+            const uint32_t a0 = __byte_perm(v0[w], v1[w], 0x5410), a1 = __byte_perm(v0[w], v1[w], 0x7632);
+            const uint32_t a2 = __byte_perm(v2[w], v3[w], 0x5410), a3 = __byte_perm(v2[w], v3[w], 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) M::mma(o[c * (S::kVV / 4) + w][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          }
+        }
+      }
+    }
+
+    // ---- join the warps ----
+    float* mine = sh_part + warp * S::kPart;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int sft = 4; sft < 32; sft <<= 1) l_run[n][j] += __shfl_xor_sync(0xffffffffu, l_run[n][j], sft);
+        const int r = n * 8 + 2 * t + j;
+        if (g == 0) {
+          mine[r] = m_run[n][j];
+          mine[S::kHeads + r] = l_run[n][j];
+        }
+#pragma unroll
+        for (int i = 0; i < S::kKSteps; ++i) {
+          // the two d of m-tile i in lane g: elements 2i and 2i + 1 of the lane's V bytes
+          constexpr int per = S::kVV / S::kElem;  // elements of one load
+          const int e = 2 * i, c = e / per;
+          const int d = c * per * 8 + g * per + e % per;
+          mine[2 * S::kHeads + r * D + d] = o[i][n][j];
+          mine[2 * S::kHeads + r * D + d + 1] = o[i][n][2 + j];
+        }
+      }
+    __syncthreads();
+    const bool whole = tile == 0 && tile_end == tiles;
+    QT* orow = static_cast<QT*>(p.out) + b * p.o_sb + static_cast<long long>(head * p.G + q0) * p.o_sh;
+    float* lrow = p.lse ? p.lse + b * p.lse_sb + head * p.G + q0 : nullptr;
+    const float vs = FP8 && p.v_scale ? p.v_scale[head] : 1.0f;
+    // parts a .. z - 1 at `parts` (stride kPart, or by contributor), joined in order
+    auto join = [&](auto&& part_of, int n_parts, bool finish, float* dst) {
+      for (int i = tid; i < nq * D; i += kThreads) {
+        const int r = i / D, d = i - r * D;
+        float mx = -INFINITY;
+        for (int w = 0; w < n_parts; ++w) mx = fmaxf(mx, __ldcg(part_of(w) + r));
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f, acc = 0.0f;
+        for (int w = 0; w < n_parts; ++w) {
+          const float* pt = part_of(w);
+          const float f = exp2_approx(__ldcg(pt + r) - ref);
+          sum = fmaf(f, __ldcg(pt + S::kHeads + r), sum);
+          acc = fmaf(f, __ldcg(pt + 2 * S::kHeads + r * D + d), acc);
+        }
+        if (finish) {
+          put(orow + r * p.o_sh + d, sum == 0.0f ? 0.0f : acc / sum * vs);
+          if (lrow && d == 0) lrow[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum) - S::kShift) * kLn2;
+        } else {
+          dst[2 * S::kHeads + r * D + d] = acc;
+          if (d == 0) dst[r] = mx, dst[S::kHeads + r] = sum;
+        }
+      }
+    };
+    // (generic loads: the warps' parts are in shared memory)
+    auto join_warps = [&](bool finish, float* dst) {
+      for (int i = tid; i < nq * D; i += kThreads) {
+        const int r = i / D, d = i - r * D;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sh_part[w * S::kPart + r]);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float* pt = sh_part + w * S::kPart;
+          const float f = exp2_approx(pt[r] - ref);
+          sum = fmaf(f, pt[S::kHeads + r], sum);
+          acc = fmaf(f, pt[2 * S::kHeads + r * D + d], acc);
+        }
+        if (finish) {
+          put(orow + r * p.o_sh + d, sum == 0.0f ? 0.0f : acc / sum * vs);
+          if (lrow && d == 0) lrow[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum) - S::kShift) * kLn2;
+        } else {
+          dst[2 * S::kHeads + r * D + d] = acc;
+          if (d == 0) dst[r] = mx, dst[S::kHeads + r] = sum;
+        }
+      }
+    };
+    if (whole) {
+      join_warps(true, nullptr);
+    } else {
+      // CTAs that hold the item's first and last tile
+      const long long last_tile = item_first + tiles - 1;
+      const int c_first = static_cast<int>(((item_first + 1) * grid - 1) / T);
+      const int c_last = static_cast<int>(((last_tile + 1) * grid - 1) / T);
+      // slot 0: the item began in an earlier CTA (this CTA's first segment); 1: it begins here
+      auto slot = [&](int c) { return p.partials + (static_cast<long long>(c) * 2 + (c == c_first ? 1 : 0)) * S::kPart; };
+      join_warps(false, slot(cta));
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) sh_last = atomicAdd(&p.counters[c_first], 1) == c_last - c_first;
+      __syncthreads();
+      if (sh_last) {
+        __threadfence();
+        join([&](int w) { return slot(c_first + w); }, c_last - c_first + 1, true, nullptr);
+        if (tid == 0) p.counters[c_first] = 0;  // the next launch starts from zero
+      }
+    }
+
+    // ---- next item ----
+    at += tile_end - tile;
+    tile = 0;
+    if (++item == per_b) {
+      item = 0;
+      if (at < t1) {
+        do {
+          ++b;
+          len = length(b);
+        } while (len == 0);
+        tiles = (len + kTile - 1) / kTile;
+      }
+    }
+  }
+}
+
+template <typename QT, bool FP8, int D, int NT, bool PAGE16>
+int launch_kernel(const AttnParams& p, int grid, cudaStream_t stream) {
+  using S = Shape<QT, FP8, D, NT>;
+  auto kernel = attn_kernel<QT, FP8, D, NT, PAGE16>;
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_dev != dev) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)) != cudaSuccess)
+      return CB_ERR_CUDA;
+    configured_dev = dev;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+constexpr int kCtasPerSm = 3;
+
+int attn_grid_limit() {
+  int sms = sm_count();
+  if (sms <= 0) sms = 148;
+  const int g = sms * kCtasPerSm;
+  return g < kMaxGrid ? g : kMaxGrid;
+}
+
+// Head blocks of 16 queries where a group has more than 8 and the output of 16
+// fits the registers (D <= 128), else of 8.
+int head_tiles(int G, int D) { return G > 8 && D <= 128 ? 2 : 1; }
+
+template <typename QT, bool FP8, int D>
+int dispatch_nt(const AttnParams& p, int nt, bool page16, int grid, cudaStream_t s) {
+  if constexpr (D <= 128) {
+    if (nt == 2)
+      return page16 ? launch_kernel<QT, FP8, D, 2, true>(p, grid, s) : launch_kernel<QT, FP8, D, 2, false>(p, grid, s);
+  }
+  return page16 ? launch_kernel<QT, FP8, D, 1, true>(p, grid, s) : launch_kernel<QT, FP8, D, 1, false>(p, grid, s);
+}
+
+template <typename QT, bool FP8>
+int dispatch_d(const AttnParams& p, int D, int nt, bool page16, int grid, cudaStream_t s) {
+  if (D == 64) return dispatch_nt<QT, FP8, 64>(p, nt, page16, grid, s);
+  if (D == 128) return dispatch_nt<QT, FP8, 128>(p, nt, page16, grid, s);
+  return dispatch_nt<QT, FP8, 256>(p, nt, page16, grid, s);
+}
+
+size_t part_bytes(int G, int D) {
+  const size_t heads = 8 * static_cast<size_t>(head_tiles(G, D));
+  return sizeof(float) * (heads * 2 + heads * D);
+}
+
+}  // namespace
+
+size_t paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D) {
+  if (Hkv < 1 || Hq < Hkv || D < 1 || D > 256) return 0;
+  return workspace_need(attn_grid_limit(), part_bytes(static_cast<int>(Hq / Hkv), static_cast<int>(D)));
+}
+
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" CB_API int cb_paged_decode_attention(const void* q, int q_dtype, const void* k_cache, const void* v_cache,
+                                                int cache_dtype, const float* k_scale, const float* v_scale,
+                                                const int* block_table, const int* seq_lens, float scale, void* out,
+                                                float* lse, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                int64_t num_pages, int64_t page_size, int64_t max_pages,
+                                                const int64_t* strides, void* workspace, size_t workspace_bytes,
+                                                cb_stream_t stream) {
+  if (B < 0 || Hq < 0 || Hkv < 0 || num_pages < 0 || page_size < 1 || max_pages < 0) return CB_ERR_INVALID_ARG;
+  if (B == 0 || Hq == 0) return CB_OK;
+  if (!q || !seq_lens || !out || !strides) return CB_ERR_INVALID_ARG;
+  if (max_pages > 0 && !block_table) return CB_ERR_INVALID_ARG;
+  if (num_pages > 0 && (!k_cache || !v_cache)) return CB_ERR_INVALID_ARG;
+  if (q_dtype != CB_DTYPE_BF16 && q_dtype != CB_DTYPE_F16) return CB_ERR_DTYPE;
+  if (cache_dtype != q_dtype && cache_dtype != CB_DTYPE_E4M3) return CB_ERR_DTYPE;
+  const bool fp8 = cache_dtype == CB_DTYPE_E4M3;
+  if (!fp8 && (k_scale || v_scale)) return CB_ERR_INVALID_ARG;
+  if ((D != 64 && D != 128 && D != 256) || Hkv < 1 || Hq % Hkv != 0) return CB_ERR_SHAPE;
+  if (B > (1 << 24) || Hq > 65536 || num_pages > 0x7fffffffLL || page_size > 0x7fffffffLL ||
+      max_pages > 0x7fffffffLL || max_pages * page_size > 0x7fffff00LL)
+    return CB_ERR_TOO_LARGE;
+  const int64_t e = fp8 ? 1 : 2;
+  for (int i = 0; i < 12; ++i)
+    if (strides[i] < 0) return CB_ERR_STRIDE;
+  // cache rows are read in 16-byte vectors
+  if (!aligned16(k_cache) || !aligned16(v_cache)) return CB_ERR_ALIGNMENT;
+  for (int i = 6; i < 12; ++i)
+    if ((strides[i] * e) % 16 != 0) return CB_ERR_ALIGNMENT;
+  const int G = static_cast<int>(Hq / Hkv);
+  const int nt = head_tiles(G, static_cast<int>(D));
+  AttnParams p = {};
+  p.q = q, p.k = k_cache, p.v = v_cache, p.table = block_table, p.lens = seq_lens;
+  p.k_scale = k_scale, p.v_scale = v_scale, p.out = out, p.lse = lse, p.scale = scale;
+  p.B = static_cast<int>(B), p.heads = static_cast<int>(Hkv), p.G = G;
+  p.blocks = (G + 8 * nt - 1) / (8 * nt);
+  p.num_pages = static_cast<int>(num_pages), p.page = static_cast<int>(page_size);
+  p.max_pages = static_cast<int>(max_pages);
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (page_size == (1LL << s)) p.page_shift = s;
+  p.q_sb = strides[0], p.q_sh = strides[1], p.o_sb = strides[2], p.o_sh = strides[3];
+  p.lse_sb = strides[4], p.table_sb = strides[5];
+  p.k_sp = strides[6] * e, p.k_ss = strides[7] * e, p.k_sh = strides[8] * e;
+  p.v_sp = strides[9] * e, p.v_ss = strides[10] * e, p.v_sh = strides[11] * e;
+  // Grid: every SM's share of CTAs, but no more than there can be tiles.
+  const long long cap = max_pages * page_size;
+  const long long most = B * Hkv * p.blocks * ((cap + kTile - 1) / kTile);
+  long long grid = attn_grid_limit();
+  if (grid > most) grid = most < 1 ? 1 : most;
+  const size_t need = workspace_need(attn_grid_limit(), part_bytes(G, static_cast<int>(D)));
+  if (!workspace || workspace_bytes < need) return CB_ERR_WORKSPACE;
+  Workspace ws = carve_workspace(workspace, static_cast<int>(grid));
+  p.status = ws.status, p.counters = ws.counters, p.partials = static_cast<float*>(ws.partials);
+  const bool page16 = page_size % 16 == 0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (q_dtype == CB_DTYPE_BF16)
+    return fp8 ? dispatch_d<__nv_bfloat16, true>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s)
+               : dispatch_d<__nv_bfloat16, false>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s);
+  return fp8 ? dispatch_d<__half, true>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s)
+             : dispatch_d<__half, false>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s);
+}

@@ -48,7 +48,8 @@ enum cb_status {
   CB_ERR_CUDA = 7,           /* a CUDA runtime/driver call failed */
   CB_ERR_DEVICE_TIMEOUT = 8, /* a bounded device-side wait expired (see cb_workspace_status) */
   CB_ERR_UNSUPPORTED = 9,    /* no kernel for this device or layout */
-  CB_ERR_TOO_LARGE = 10      /* size beyond a documented maximum */
+  CB_ERR_TOO_LARGE = 10,     /* size beyond a documented maximum */
+  CB_ERR_DEVICE_INDEX = 11   /* a cache slot, page index or length was outside the cache (see cb_workspace_status) */
 };
 
 /* ---- dtype codes -------------------------------------------------------- */
@@ -58,11 +59,26 @@ enum cb_dtype {
   CB_DTYPE_F32 = 2,
   CB_DTYPE_I8 = 3,
   CB_DTYPE_U8 = 4,
-  CB_DTYPE_I32 = 5
+  CB_DTYPE_I32 = 5,
+  CB_DTYPE_E4M3 = 6 /* fp8 e4m3 (paged caches) */
 };
 
 /* ---- operation codes (for cb_workspace_bytes) --------------------------- */
-enum cb_op { CB_OP_W8A8 = 0, CB_OP_W4A16 = 1, CB_OP_W4A4 = 2, CB_OP_NVFP4 = 3 };
+enum cb_op {
+  CB_OP_W8A8 = 0,
+  CB_OP_W4A16 = 1,
+  CB_OP_W4A4 = 2,
+  CB_OP_NVFP4 = 3,
+  CB_OP_FP8_BLOCK = 4,
+  CB_OP_PAGED_ATTENTION = 5 /* M = query heads, N = key-value heads, K = head size */
+};
+
+/* ---- output forms of cb_add_rmsnorm_quant ------------------------------- */
+enum cb_norm_mode {
+  CB_NORM_INT8 = 0,     /* int8, one scale per row */
+  CB_NORM_FP8 = 1,      /* e4m3, one scale per row */
+  CB_NORM_FP8_BLOCK = 2 /* e4m3, one scale per 128 elements of a row */
+};
 
 /* ---- int4 weight layouts ------------------------------------------------ */
 enum cb_w4_layout {
@@ -93,9 +109,10 @@ CB_API int cb_device_sm_count(void);
 CB_API size_t cb_workspace_bytes(int op, int64_t batch, int64_t M, int64_t N, int64_t K);
 
 /* Copies the workspace status word to *device_status after synchronizing the
-   stream. Returns CB_ERR_DEVICE_TIMEOUT if a kernel recorded an expired wait
-   (and then clears the word and the workspace's arrival counters, which a
-   kernel that gave up a wait may leave behind), CB_OK otherwise. */
+   stream. Returns CB_ERR_DEVICE_TIMEOUT if a kernel recorded an expired wait,
+   else CB_ERR_DEVICE_INDEX if one met a cache slot, page index or length outside
+   the cache (and then clears the word and the workspace's arrival counters,
+   which a kernel that gave up a wait may leave behind), CB_OK otherwise. */
 CB_API int cb_workspace_status(void* workspace, int* device_status, cb_stream_t stream);
 
 /* Failure-detection test hook (no counterpart in the reference). With a
@@ -360,6 +377,85 @@ CB_API int cb_repack_w8_kmajor(const int8_t* src_kn, int8_t* dst_nk, int64_t bat
 CB_API int cb_rmsnorm_quant_i8(const void* x, int x_dtype, const void* weight, int w_dtype, float eps, int64_t rows,
                                int64_t H, int64_t x_sm, int8_t* q, int64_t q_sm, float* scale, void* y_out,
                                int64_t y_sm, cb_stream_t stream);
+
+/* ---- The rest of a quantized decoder layer (no counterpart kernels in the
+ * reference, whose dense path stops at the projections) ------------------- */
+
+/* Residual addition + RMSNorm + 8-bit output. Per row of x [rows, H] (f16/bf16),
+   in fp32: h = x + residual; r = 1 / sqrt(mean(h^2) + eps); u = h * weight;
+   step = max(amax |u| / Q, 2^-100) over the row (CB_NORM_INT8, Q = 127;
+   CB_NORM_FP8, Q = 448) or over each 128 elements (CB_NORM_FP8_BLOCK, Q = 448);
+   q = u / step (int8: rounded half away from zero; e4m3: to nearest even);
+   scale = step * r. q * scale is the normalised row; r divides out of q. The norm
+   takes h before it is rounded. residual: like x, or null; h_out (nullable, only
+   with a residual) receives h in x's type and may be x's or the residual's own
+   buffer. weight: [H] f16, bf16 or f32. scale: one per row (scale[row * s_sm]) or
+   ceil(H / 128) per row, contiguous. A NaN in a row makes that row's scales
+   NaN; an infinity makes its group's scale NaN and the row's other scales zero. */
+CB_API int cb_add_rmsnorm_quant(const void* x, const void* residual, int x_dtype, const void* weight, int w_dtype,
+                                float eps, int64_t rows, int64_t H, int64_t x_sm, int64_t r_sm, int mode, void* q,
+                                int64_t q_sm, float* scale, int64_t s_sm, void* h_out, int64_t h_sm,
+                                cb_stream_t stream);
+
+/* e4m3 quantization of a [batch, M, K] (f16/bf16) with one scale per 128 elements
+   of a row: scale[b, m, kb] = max(amax / 448, 1 / (448 * 512)), q = a / scale. */
+CB_API int cb_quant_act_fp8_block(const void* a, int a_dtype, int64_t batch, int64_t M, int64_t K, int64_t a_sb,
+                                  int64_t a_sm, uint8_t* q, int64_t q_sb, int64_t q_sm, float* scale, int64_t s_sb,
+                                  int64_t s_sm, cb_stream_t stream);
+
+/* out[b, m, n] = cvt( sum_kb a_scale[b, m, kb] * w_scale[b, n / 128, kb] *
+                       (sum_{k in kb} aq[b, m, k] * w[b, n, k]) (+ bias[b, n]) ),
+   kb the blocks of 128 along K (the last may be shorter), fp32 accumulation.
+   aq: e4m3 [batch, M, K], w: e4m3 [batch, N, K] (K-major), K % 16 == 0, 16-byte
+   aligned rows. strides (elements): {aq_b, aq_m, w_b, w_n, out_b, out_m,
+   a_scale_b, a_scale_m, w_scale_b, w_scale_n, bias_b}; the scales are contiguous
+   along kb. bias: [batch, N] f16, bf16 or f32, or null. Workspace:
+   cb_workspace_bytes(CB_OP_FP8_BLOCK, ...). */
+CB_API int cb_fp8_block_gemm(const uint8_t* aq, const float* a_scale, const uint8_t* w, const float* w_scale,
+                             const void* bias, int bias_dtype, void* out, int out_dtype, int64_t batch, int64_t M,
+                             int64_t N, int64_t K, const int64_t* strides, void* workspace, size_t workspace_bytes,
+                             cb_stream_t stream);
+/* cb_quant_act_fp8_block of a (f16/bf16, strides a_sb, a_sm) into q and scale,
+   then cb_fp8_block_gemm on them (strides describe q and scale). */
+CB_API int cb_fp8_block_gemm_dynamic(const void* a, int a_dtype, int64_t a_sb, int64_t a_sm, uint8_t* q, float* scale,
+                                     const uint8_t* w, const float* w_scale, const void* bias, int bias_dtype,
+                                     void* out, int out_dtype, int64_t batch, int64_t M, int64_t N, int64_t K,
+                                     const int64_t* strides, void* workspace, size_t workspace_bytes,
+                                     cb_stream_t stream);
+
+/* Writes new keys and values [T, heads, D] (f16/bf16) into paged caches of
+   num_pages x page_size slots: token t goes to slot slots[t] (int32, or int64 with
+   slots_i64), page slot / page_size. cache_dtype: f16, bf16 or e4m3; an e4m3 cache
+   stores row / scale[head], saturated (k_scale, v_scale: [heads] fp32, null = 1).
+   A negative slot skips its token; a slot past the cache is skipped too and sets
+   bit 2 of *status (nullable; a workspace's first word). Two tokens with one slot
+   leave either. strides (elements): {k_t, k_h, kcache_page, kcache_slot,
+   kcache_head} and the same five for v. */
+CB_API int cb_paged_kv_append(const void* k, const void* v, int dtype, void* k_cache, void* v_cache, int cache_dtype,
+                              const float* k_scale, const float* v_scale, const void* slots, int slots_i64, int64_t T,
+                              int64_t heads, int64_t D, int64_t num_pages, int64_t page_size, const int64_t* strides,
+                              int* status, cb_stream_t stream);
+
+/* Attention of one new token per sequence over a paged cache:
+     out[b, h] = sum_l softmax_l(scale * q[b, h] . k_l) v_l,  lse[b, h] = log sum_l exp(scale * q . k_l)
+   over the seq_lens[b] tokens l of sequence b; token l lies in page
+   block_table[b, l / page_size], slot l % page_size; query head h reads kv head
+   h / (Hq / Hkv). q, out: [B, Hq, D] f16/bf16, D 64, 128 or 256; the caches have
+   q's type or are e4m3 with k_scale, v_scale [Hkv] fp32 (null = 1). lse
+   (nullable): fp32 [B, Hq], natural logarithm. A sequence of length 0 gives zeros
+   and an lse of -inf. Slots past a sequence's length are not read, whatever they
+   hold. A page index outside the cache counts as masked, a length outside the
+   table is clamped; both set bit 2 of the workspace's status word. strides
+   (elements): {q_b, q_h, out_b, out_h, lse_b, table_b, kcache_page, kcache_slot,
+   kcache_head, vcache_page, vcache_slot, vcache_head}; the caches' rows are
+   16-byte aligned. Workspace: cb_workspace_bytes(CB_OP_PAGED_ATTENTION, B, Hq,
+   Hkv, D). */
+CB_API int cb_paged_decode_attention(const void* q, int q_dtype, const void* k_cache, const void* v_cache,
+                                     int cache_dtype, const float* k_scale, const float* v_scale,
+                                     const int* block_table, const int* seq_lens, float scale, void* out, float* lse,
+                                     int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages,
+                                     int64_t page_size, int64_t max_pages, const int64_t* strides, void* workspace,
+                                     size_t workspace_bytes, cb_stream_t stream);
 
 /* ---- One-shot all-reduce over NVLink peer memory (tensor-parallel projections) ----
  * No counterpart in the reference, which has no multi-GPU code: it replaces the
