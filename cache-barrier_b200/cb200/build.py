@@ -5,6 +5,9 @@
 ``compute_100a/sm_100a`` and links one shared library next to this file. The
 library exports the C ABI declared in ``include/cb200.h`` and links the CUDA
 runtime statically, so it loads with ``ctypes`` alone.
+
+``csrc/torch_binding.cpp`` (the native torch layer of the decoder-layer operators)
+is compiled with the host compiler against the installed torch into ``_native.so``.
 """
 
 from __future__ import annotations
@@ -22,6 +25,8 @@ CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 OBJ_DIR = os.path.join(PKG_ROOT, "_build")
 LIB_PATH = os.path.join(HERE, "libcb200.so")
+NATIVE_SRC = os.path.join(CSRC, "torch_binding.cpp")
+NATIVE_PATH = os.path.join(HERE, "_native.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -52,8 +57,25 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _native_command() -> list[str]:
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: the native torch layer cannot be built")
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + sysconfig.get_paths()["include"],
+            "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            "-I" + os.path.join(cuda, "include"), "-I" + INCLUDE, NATIVE_SRC, "-o", NATIVE_PATH,
+            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
-    """Compile (if stale) and return the path of ``libcb200.so``."""
+    """Compile (if stale) the library and the native torch layer; the path of ``libcb200.so``."""
     nvcc = _nvcc()
     os.makedirs(OBJ_DIR, exist_ok=True)
     headers = _headers()
@@ -73,6 +95,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
             sys.stdout.write(r.stdout + r.stderr)
         return cmd
 
+    if force or _stale(NATIVE_PATH, [NATIVE_SRC, os.path.join(INCLUDE, "cb200.h")]):
+        jobs.append(_native_command())
     if jobs:
         with cf.ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
             list(ex.map(run, jobs))

@@ -12,8 +12,6 @@ profiling/w8a8/w8a8_bmm.py:118-140).
 from __future__ import annotations
 
 import ctypes
-import functools
-import math
 import threading
 
 import torch
@@ -73,6 +71,7 @@ class WorkspacePool:
     def __init__(self):
         self._bufs = {}
         self._lock = threading.Lock()
+        self._native = None  # the native layer, once it holds addresses of these buffers
 
     def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
         key = (device.index, _stream(device))
@@ -84,7 +83,16 @@ class WorkspacePool:
                     size = max(size, 2 * buf.numel())
                 buf = torch.zeros(size, dtype=torch.uint8, device=device)
                 self._bufs[key] = buf
+                if self._native is not None:
+                    self._native.set_workspace(*key, buf.data_ptr(), buf.numel())
             return buf
+
+    def share(self, nbytes: int, device: torch.device, native) -> None:
+        """``get``, and the buffer's address to the native layer. That layer asks again
+        where it needs more bytes; ``get`` tells it when a buffer is replaced."""
+        self._native = native
+        buf = self.get(nbytes, device)
+        native.set_workspace(device.index, _stream(device), buf.data_ptr(), buf.numel())
 
     def check_status(self, device: torch.device | None = None) -> int:
         """Synchronising read of the device status word of every buffer on device."""
@@ -533,35 +541,24 @@ def nvfp4_gemm(a: torch.Tensor, a_sf: torch.Tensor, b: torch.Tensor, b_sf: torch
 # ---------------------------------------------------------------------------
 FP8_BLOCK = 128  # elements of K per scale of the block-scaled GEMM
 
-_NORM_MODES = {"int8": L.CB_NORM_INT8, "fp8": L.CB_NORM_FP8, "fp8_block": L.CB_NORM_FP8_BLOCK}
-_ACT_CODE = {torch.float16: L.CB_DTYPE_F16, torch.bfloat16: L.CB_DTYPE_BF16}
-_CACHE_CODE = {**_ACT_CODE, torch.float8_e4m3fn: L.CB_DTYPE_E4M3}
+_native = None
 
 
-@functools.lru_cache(maxsize=4096)
-def _workspace_need(device_index: int, op: int, batch: int, M: int, N: int, K: int) -> int:
-    with torch.cuda.device(device_index):
-        return workspace_bytes(op, batch, M, N, K)
-
-
-def _one_device(first: torch.Tensor, *rest) -> None:
-    d = first.device
-    if d.type != "cuda":
-        raise ValueError("all tensors must be CUDA tensors (the kernels run only on the GPU)")
-    for t in rest:
-        if t is not None and t.device != d:
-            raise ValueError(f"all tensors must be on one device, got {t.device} and {d}")
-
-
-def _act_code(t: torch.Tensor, name: str) -> int:
-    code = _ACT_CODE.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{name} must be float16 or bfloat16, got {t.dtype}")
-    return code
-
-
-def _fp8(t: torch.Tensor) -> bool:
-    return t.dtype == torch.float8_e4m3fn or t.dtype == torch.uint8
+def _N():
+    """The native torch layer (``csrc/torch_binding.cpp``), which checks the tensors and calls the library."""
+    global _native
+    if _native is None:
+        lib = L.load()
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise RuntimeError(f"cb200/_native.so does not load ({e}); build it with cb200.build.build()") from e
+        names = ("cb_add_rmsnorm_quant", "cb_quant_act_fp8_block", "cb_fp8_block_gemm", "cb_fp8_block_gemm_dynamic",
+                 "cb_paged_kv_append", "cb_paged_decode_attention", "cb_workspace_bytes")
+        module.init({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, L.check,
+                    lambda nbytes, index: POOL.share(nbytes, torch.device("cuda", index), module))
+        _native = module
+    return _native
 
 
 def add_rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -581,115 +578,14 @@ def add_rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
     tensor (updated in place). A row that holds a
     NaN gets NaN scales; an infinity makes its group's scale NaN, the row's others zero.
     """
-    if x.dim() != 2 or x.stride(1) != 1:
-        raise ValueError("x must be [rows, H], contiguous along H")
-    _one_device(x, weight, residual, q, s, h)
-    code = _act_code(x, "x")
-    rows, H = x.shape
-    kind = _NORM_MODES.get(mode)
-    if kind is None:
-        raise ValueError(f"mode must be one of {sorted(_NORM_MODES)}")
-    if weight.dim() != 1 or weight.shape[0] != H or not weight.is_contiguous():
-        raise ValueError("weight must be a contiguous [H] tensor")
-    if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.stride(1) != 1:
-            raise ValueError("residual must be like x")
-        if h is None:
-            h = torch.empty(rows, H, dtype=x.dtype, device=x.device)
-        elif h.shape != x.shape or h.dtype != x.dtype or h.stride(1) != 1:
-            raise ValueError("h must be like x")
-    elif h is not None:
-        raise ValueError("h is the sum with the residual: give one")
-    q_dtype = torch.int8 if kind == L.CB_NORM_INT8 else torch.float8_e4m3fn
-    if q is None:
-        q = torch.empty(rows, H, dtype=q_dtype, device=x.device)
-    elif q.shape != x.shape or q.dtype != q_dtype or q.stride(1) != 1:
-        raise ValueError(f"q must be {q_dtype} [rows, H], contiguous along H")
-    block = kind == L.CB_NORM_FP8_BLOCK
-    if s is None:
-        s = torch.empty((rows, -(-H // FP8_BLOCK)) if block else (rows,), dtype=torch.float32, device=x.device)
-    elif block:
-        if s.dtype != torch.float32 or s.shape != (rows, -(-H // FP8_BLOCK)) or s.stride(1) != 1:
-            raise ValueError("s must be fp32 [rows, ceil(H / 128)], contiguous along the blocks")
-    elif s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != rows:
-        raise ValueError("s must be fp32 [rows]")
-    code = L.load().cb_add_rmsnorm_quant(
-        x.data_ptr(), None if residual is None else residual.data_ptr(), code, weight.data_ptr(),
-        dtype_code(weight.dtype), eps, rows, H, x.stride(0), 0 if residual is None else residual.stride(0), kind,
-        q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), None if h is None else h.data_ptr(),
-        0 if h is None else h.stride(0), _stream(x.device))
-    if code:
-        L.check("cb_add_rmsnorm_quant", code)
-    return q, s, h
-
-
-def _block_outputs(a: torch.Tensor, q, s):
-    """q and s of a block-quantized ``a`` ([M, K] or [B, M, K]), checked or allocated."""
-    K = a.shape[-1]
-    s_shape = (*a.shape[:-1], -(-K // FP8_BLOCK))
-    if q is None:
-        q = torch.empty(a.shape, dtype=torch.float8_e4m3fn, device=a.device)
-    elif q.shape != a.shape or not _fp8(q) or q.stride(-1) != 1:
-        raise ValueError("q must be float8_e4m3fn like a, contiguous along K")
-    if s is None:
-        s = torch.empty(s_shape, dtype=torch.float32, device=a.device)
-    elif s.shape != s_shape or s.dtype != torch.float32 or s.stride(-1) != 1:
-        raise ValueError("s must be fp32 [.., M, ceil(K / 128)], contiguous along the blocks")
-    return q, s
+    return _N().add_rmsnorm_quant(x, weight, eps, residual, mode, q, s, h)
 
 
 def quant_act_fp8_block(a: torch.Tensor, q: torch.Tensor | None = None, s: torch.Tensor | None = None):
     """e4m3 quantization of ``a`` ([M, K] or [B, M, K], f16/bf16) with one scale per
     128 elements of a row: ``s = max(amax / 448, 1 / (448 * 512))``, ``q = a / s``.
     Returns ``(q, s)``, s fp32 ``[.., M, ceil(K / 128)]``."""
-    if a.dim() not in (2, 3) or a.stride(-1) != 1:
-        raise ValueError("a must be [M, K] or [B, M, K], contiguous along K")
-    _one_device(a, q, s)
-    code = _act_code(a, "a")
-    q, s = _block_outputs(a, q, s)
-    three = a.dim() == 3
-    code = L.load().cb_quant_act_fp8_block(
-        a.data_ptr(), code, a.shape[0] if three else 1, a.shape[-2], a.shape[-1], a.stride(0) if three else 0,
-        a.stride(-2), q.data_ptr(), q.stride(0) if three else 0, q.stride(-2), s.data_ptr(), s.stride(0) if three else 0,
-        s.stride(-2), _stream(a.device))
-    if code:
-        L.check("cb_quant_act_fp8_block", code)
-    return q, s
-
-
-def _block_gemm_args(a, w_nk, w_scale, a_scale, out, out_dtype, bias, aq):
-    """Checks of the block-scaled GEMM; (out, batch, M, N, K, strides, bias strides' code)."""
-    three = aq.dim() == 3
-    if aq.dim() not in (2, 3) or w_nk.dim() != aq.dim():
-        raise ValueError("a must be [M, K] or [B, M, K] and w_nk [N, K] or [B, N, K]")
-    M, K = aq.shape[-2], aq.shape[-1]
-    N = w_nk.shape[-2]
-    B = aq.shape[0] if three else 1
-    if w_nk.shape[-1] != K or (three and w_nk.shape[0] != B):
-        raise ValueError(f"shape mismatch: a {tuple(aq.shape)} vs w {tuple(w_nk.shape)}")
-    if not _fp8(w_nk) or w_nk.stride(-1) != 1:
-        raise ValueError("w_nk must be float8_e4m3fn, contiguous along K (K-major [N, K])")
-    KB, NB = -(-K // FP8_BLOCK), -(-N // FP8_BLOCK)
-    if w_scale.dtype != torch.float32 or w_scale.shape != ((B, NB, KB) if three else (NB, KB)) or w_scale.stride(-1) != 1:
-        raise ValueError("w_scale must be fp32 [.., ceil(N / 128), ceil(K / 128)], contiguous along K")
-    shape = (B, M, N) if three else (M, N)
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=aq.device)
-    elif out.shape != shape or out.stride(-1) != 1:
-        raise ValueError("out must be [.., M, N], contiguous along N")
-    b_code, b_ptr, b_sb = 0, None, 0
-    if bias is not None:
-        if bias.shape[-1] != N or bias.stride(-1) != 1 or bias.dim() not in (1, 2) or (bias.dim() == 2 and bias.shape[0] != B):
-            raise ValueError("bias must be [N] or [B, N], contiguous along N")
-        b_code, b_ptr, b_sb = dtype_code(bias.dtype), bias.data_ptr(), bias.stride(0) if bias.dim() == 2 else 0
-    if three:
-        st = (ctypes.c_int64 * 11)(aq.stride(0), aq.stride(1), w_nk.stride(0), w_nk.stride(1), out.stride(0),
-                                   out.stride(1), a_scale.stride(0), a_scale.stride(1), w_scale.stride(0),
-                                   w_scale.stride(1), b_sb)
-    else:
-        st = (ctypes.c_int64 * 11)(0, aq.stride(0), 0, w_nk.stride(0), 0, out.stride(0), 0, a_scale.stride(0), 0,
-                                   w_scale.stride(0), b_sb)
-    return out, B, M, N, K, st, b_ptr, b_code
+    return _N().quant_act_fp8_block(a, q, s)
 
 
 def fp8_block_gemm(aq: torch.Tensor, w_nk: torch.Tensor, a_scale: torch.Tensor, w_scale: torch.Tensor,
@@ -703,21 +599,7 @@ def fp8_block_gemm(aq: torch.Tensor, w_nk: torch.Tensor, a_scale: torch.Tensor, 
     (``wformat.quantize_fp8_block``). K is a multiple of 16; blocks at the ends of N
     and K may be partial. out: f16, bf16 or f32, rounded once from fp32.
     """
-    _one_device(aq, w_nk, a_scale, w_scale, out, bias)
-    if not _fp8(aq) or aq.stride(-1) != 1:
-        raise ValueError("aq must be float8_e4m3fn, contiguous along K")
-    if a_scale.dtype != torch.float32 or a_scale.shape != (*aq.shape[:-1], -(-aq.shape[-1] // FP8_BLOCK)) or \
-            a_scale.stride(-1) != 1:
-        raise ValueError("a_scale must be fp32 [.., M, ceil(K / 128)], contiguous along the blocks")
-    out, B, M, N, K, st, b_ptr, b_code = _block_gemm_args(aq, w_nk, w_scale, a_scale, out, out_dtype, bias, aq)
-    dev = aq.device
-    ws = POOL.get(_workspace_need(dev.index, L.CB_OP_FP8_BLOCK, B, M, N, K), dev)
-    code = L.load().cb_fp8_block_gemm(aq.data_ptr(), a_scale.data_ptr(), w_nk.data_ptr(), w_scale.data_ptr(), b_ptr,
-                                      b_code, out.data_ptr(), dtype_code(out.dtype), B, M, N, K, st, ws.data_ptr(),
-                                      ws.numel(), _stream(dev))
-    if code:
-        L.check("cb_fp8_block_gemm", code)
-    return out
+    return _N().fp8_block_gemm(aq, w_nk, a_scale, w_scale, out, out_dtype, bias)
 
 
 def fp8_block_gemm_dynamic(a: torch.Tensor, w_nk: torch.Tensor, w_scale: torch.Tensor, q: torch.Tensor | None = None,
@@ -726,40 +608,7 @@ def fp8_block_gemm_dynamic(a: torch.Tensor, w_nk: torch.Tensor, w_scale: torch.T
     """``quant_act_fp8_block(a)`` into q and s (allocated unless given), then ``fp8_block_gemm``.
 
     out: a's type unless ``out_dtype`` or ``out`` says otherwise."""
-    if a.dim() not in (2, 3) or a.stride(-1) != 1:
-        raise ValueError("a must be [M, K] or [B, M, K], contiguous along K")
-    _one_device(a, w_nk, w_scale, q, s, out, bias)
-    a_code = _act_code(a, "a")
-    q, s = _block_outputs(a, q, s)
-    out, B, M, N, K, st, b_ptr, b_code = _block_gemm_args(a, w_nk, w_scale, s, out, out_dtype or a.dtype, bias, q)
-    dev = a.device
-    ws = POOL.get(_workspace_need(dev.index, L.CB_OP_FP8_BLOCK, B, M, N, K), dev)
-    code = L.load().cb_fp8_block_gemm_dynamic(
-        a.data_ptr(), a_code, a.stride(0) if a.dim() == 3 else 0, a.stride(-2), q.data_ptr(), s.data_ptr(),
-        w_nk.data_ptr(), w_scale.data_ptr(), b_ptr, b_code, out.data_ptr(), dtype_code(out.dtype), B, M, N, K, st,
-        ws.data_ptr(), ws.numel(), _stream(dev))
-    if code:
-        L.check("cb_fp8_block_gemm_dynamic", code)
-    return out
-
-
-def _cache_args(k_cache, v_cache, k_scale, v_scale):
-    """Checks of a paged cache pair; (dtype code, pages, page size, heads, D)."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
-        raise ValueError("k_cache and v_cache must be alike: [pages, page_size, heads, D]")
-    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
-        raise ValueError("caches must be contiguous along D")
-    code = _CACHE_CODE.get(k_cache.dtype)
-    if code is None:
-        raise ValueError(f"caches must be float16, bfloat16 or float8_e4m3fn, got {k_cache.dtype}")
-    heads = k_cache.shape[2]
-    for sc in (k_scale, v_scale):
-        if sc is not None:
-            if code != L.CB_DTYPE_E4M3:
-                raise ValueError("k_scale and v_scale belong to float8_e4m3fn caches")
-            if sc.dtype != torch.float32 or sc.shape != (heads,) or not sc.is_contiguous():
-                raise ValueError("k_scale and v_scale must be contiguous fp32 [heads]")
-    return code, k_cache.shape[0], k_cache.shape[1], heads, k_cache.shape[3]
+    return _N().fp8_block_gemm_dynamic(a, w_nk, w_scale, q, s, out, out_dtype, bias)
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -772,25 +621,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     slot ``slots[t] % page_size``; a negative slot skips its token. An e4m3 cache
     stores ``k / k_scale[head]``, saturated. A slot past the cache is skipped and
     shows in ``device_status``. Two tokens with the same slot leave either of them."""
-    _one_device(k, v, k_cache, v_cache, slots, k_scale, v_scale)
-    code = _act_code(k, "k")
-    c_code, pages, page, heads, D = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    if k.dim() != 3 or k.shape[1] != heads or k.shape[2] != D or v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError("k and v must be alike: [T, heads, D] with the caches' heads and D")
-    if k.stride(2) != 1 or v.stride(2) != 1:
-        raise ValueError("k and v must be contiguous along D")
-    T = k.shape[0]
-    if slots.shape != (T,) or slots.dtype not in (torch.int32, torch.int64) or (T > 1 and slots.stride(0) != 1):
-        raise ValueError("slots must be a contiguous int32 or int64 [T] tensor")
-    dev = k.device
-    st = (ctypes.c_int64 * 10)(k.stride(0), k.stride(1), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                               v.stride(0), v.stride(1), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2))
-    status = POOL.get(1, dev)
-    code = L.load().cb_paged_kv_append(
-        k.data_ptr(), v.data_ptr(), code, k_cache.data_ptr(), v_cache.data_ptr(), c_code, _ptr(k_scale), _ptr(v_scale),
-        slots.data_ptr(), slots.dtype == torch.int64, T, heads, D, pages, page, st, status.data_ptr(), _stream(dev))
-    if code:
-        L.check("cb_paged_kv_append", code)
+    _N().paged_kv_append(k, v, k_cache, v_cache, slots, k_scale, v_scale)
 
 
 def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -809,37 +640,7 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     sequence of length 0 gives zeros and -inf. Page indices or lengths outside the
     cache are masked or clamped and show in ``device_status``.
     """
-    _one_device(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, out, lse)
-    code = _act_code(q, "q")
-    c_code, pages, page, Hkv, D = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1:
-        raise ValueError("q must be [B, Hq, D], contiguous along D, with the caches' D")
-    B, Hq = q.shape[0], q.shape[1]
-    if c_code != code and c_code != L.CB_DTYPE_E4M3:
-        raise ValueError("the caches must have q's type or be float8_e4m3fn")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [B, max_pages], contiguous along the pages")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or (B > 1 and seq_lens.stride(0) != 1):
-        raise ValueError("seq_lens must be a contiguous int32 [B] tensor")
-    if out is None:
-        out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
-        raise ValueError("out must be like q")
-    if lse is not None and (lse.shape != (B, Hq) or lse.dtype != torch.float32 or lse.stride(1) != 1):
-        raise ValueError("lse must be fp32 [B, Hq], contiguous along Hq")
-    dev = q.device
-    st = (ctypes.c_int64 * 12)(q.stride(0), q.stride(1), out.stride(0), out.stride(1), 0 if lse is None else lse.stride(0),
-                               block_table.stride(0), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                               v_cache.stride(0), v_cache.stride(1), v_cache.stride(2))
-    ws = POOL.get(_workspace_need(dev.index, L.CB_OP_PAGED_ATTENTION, 0, Hq, Hkv, D), dev)
-    code = L.load().cb_paged_decode_attention(
-        q.data_ptr(), code, k_cache.data_ptr(), v_cache.data_ptr(), c_code, _ptr(k_scale), _ptr(v_scale),
-        block_table.data_ptr(), seq_lens.data_ptr(), 1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(),
-        _ptr(lse), B, Hq, Hkv, D, pages, page, block_table.shape[1], st, ws.data_ptr(), ws.numel(), _stream(dev))
-    if code:
-        L.check("cb_paged_decode_attention", code)
-    return out
+    return _N().paged_decode_attention(q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale, out, lse)
 
 
 def device_status(device: torch.device | None = None) -> int:
