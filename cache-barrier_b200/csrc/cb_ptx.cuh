@@ -84,6 +84,28 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// mbar_wait for hand-offs on a kernel's critical path: %globaltimer (about a
+// microsecond a read) and the abort flag are looked at once per 256 polls, so a
+// phase that completes between two of those looks is seen at once. Same bound,
+// same result on expiry.
+__device__ __forceinline__ bool mbar_wait_quick(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                int* status) {
+  unsigned long long t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (abort_flag && *abort_flag) return false;
+    const unsigned long long now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      if (abort_flag) *abort_flag = 1;
+      if (status) atomicOr(status, CB_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
 // Acquire load of a counter in global memory (pairs with a writer's fence +
 // atomic increment).
 __device__ __forceinline__ int ld_acquire_gpu(const int* ptr) {

@@ -15,6 +15,7 @@
 #include "cb_gemm_common.cuh"
 #include "cb_internal.h"
 #include "cb_ptx.cuh"
+#include "fp8_block.h"
 
 namespace cb {
 namespace {
@@ -113,7 +114,7 @@ int launch_block_gemm(const BlockGemmParams& p, int64_t batch, cudaStream_t stre
 
 size_t fp8_block_workspace_bytes(int64_t M) {
   (void)M;
-  return kWsHeader + kWsCounters;
+  return block_gemm_tc_workspace();
 }
 
 }  // namespace cb
@@ -144,6 +145,17 @@ extern "C" CB_API int cb_fp8_block_gemm(const uint8_t* aq, const float* a_scale,
       (batch > 1 && (strides[0] % 16 || strides[2] % 16)))
     return CB_ERR_ALIGNMENT;
   if (!workspace || workspace_bytes < fp8_block_workspace_bytes(M)) return CB_ERR_WORKSPACE;
+  cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+  if (M > 16) {
+    BlockGemmArgs L = {};
+    L.a = aq, L.a_scale = a_scale, L.w = w, L.w_scale = w_scale, L.bias = bias, L.bias_dtype = bias_dtype;
+    L.out = out, L.out_dtype = out_dtype, L.batch = batch, L.M = M, L.N = N, L.K = K;
+    L.a_sb = strides[0], L.a_sm = strides[1], L.w_sb = strides[2], L.w_sn = strides[3], L.o_sb = strides[4];
+    L.o_sm = strides[5], L.as_sb = strides[6], L.as_sm = strides[7], L.ws_sb = strides[8], L.ws_sn = strides[9];
+    L.b_sb = strides[10];
+    L.workspace = workspace;
+    return block_gemm_pair_eligible(L) ? launch_block_gemm_pair(L, cs) : launch_block_gemm_tc(L, cs);
+  }
   BlockGemmParams p = {};
   p.a = aq, p.a_scale = a_scale, p.w = w, p.w_scale = w_scale, p.bias = bias, p.bias_dtype = bias_dtype;
   p.out = out, p.out_dtype = out_dtype;
@@ -151,7 +163,7 @@ extern "C" CB_API int cb_fp8_block_gemm(const uint8_t* aq, const float* a_scale,
   p.a_sb = strides[0], p.a_sm = strides[1], p.w_sb = strides[2], p.w_sn = strides[3], p.o_sb = strides[4];
   p.o_sm = strides[5], p.as_sb = strides[6], p.as_sm = strides[7], p.ws_sb = strides[8], p.ws_sn = strides[9];
   p.b_sb = strides[10];
-  return launch_block_gemm(p, batch, reinterpret_cast<cudaStream_t>(stream));
+  return launch_block_gemm(p, batch, cs);
 }
 
 extern "C" CB_API int cb_fp8_block_gemm_dynamic(const void* a, int a_dtype, int64_t a_sb, int64_t a_sm, uint8_t* q,

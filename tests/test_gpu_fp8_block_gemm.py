@@ -89,6 +89,24 @@ def test_types_and_bias(cuda_device, M, N, K, out_dtype):
     assert torch.equal(again.view(torch.uint8), out.view(torch.uint8))  # the sums have one order
 
 
+@pytest.mark.parametrize("B,M,N,K", [(1, 4500, 5000, 272), (1, 8000, 2560, 1040), (2, 1100, 8200, 128), (1, 300, 40000, 400),
+                                     (1, 40000, 300, 1536)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_many_tiles(cuda_device, B, M, N, K, out_dtype):
+    """Problems with many tiles, ragged in every direction; the reference runs in 64 bits on the device."""
+    from cb200 import ops
+    a, w, a_s, w_s = (t.to(cuda_device) for t in _squeeze(B, *_make(B, M, N, K, M)))
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    out = ops.fp8_block_gemm(a, w, a_s, w_s, out_dtype=out_dtype, bias=bias)
+    y, S = _exact(a, w, a_s, w_s, bias)
+    assert torch.all((out.double() - y).abs() <= U[out_dtype] * y.abs() + 2.0 ** -12 * S)
+    assert torch.equal(ops.fp8_block_gemm(a, w, a_s, w_s, out_dtype=out_dtype, bias=bias), out)
+    odd = torch.full((*out.shape[:-1], N + 1), 3.0, dtype=out_dtype, device=cuda_device)  # rows off the 16-byte grid
+    ops.fp8_block_gemm(a, w, a_s, w_s, out=odd[..., :N], bias=bias)
+    assert torch.equal(odd[..., :N], out) and torch.all(odd[..., N] == 3.0)
+    assert ops.device_status(cuda_device) == 0
+
+
 @pytest.mark.parametrize("M", [1, 3, 20, 150])
 def test_batches_and_strides(cuda_device, M):
     from cb200 import ops
