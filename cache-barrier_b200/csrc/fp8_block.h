@@ -21,6 +21,8 @@ struct BlockGemmArgs {
 
 bool block_gemm_pair_eligible(const BlockGemmArgs& L);
 int launch_block_gemm_pair(const BlockGemmArgs& L, cudaStream_t stream);
+int launch_block_gemm_decode(const BlockGemmArgs& L, cudaStream_t stream);
+size_t block_gemm_decode_workspace();
 int launch_block_gemm_tc(const BlockGemmArgs& L, cudaStream_t stream);
 size_t block_gemm_tc_workspace();
 

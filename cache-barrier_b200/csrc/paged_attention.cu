@@ -128,8 +128,9 @@ struct Math<false> {
 
 // Two e4m3 values (exact) as f16x2.
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+  uint32_t d;
+  asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(d) : "r"(two));
+  return d;
 }
 
 __device__ __forceinline__ float q_val(const __half* p) { return __half2float(*p); }
