@@ -19,7 +19,9 @@ struct BlockGemmArgs {
   void* workspace;
 };
 
-bool block_gemm_pair_eligible(const BlockGemmArgs& L);
+// 128-element blocks of K that the busiest CTA (pair) works through.
+long long block_gemm_pair_blocks(const BlockGemmArgs& L);
+long long block_gemm_tc_blocks(const BlockGemmArgs& L);
 int launch_block_gemm_pair(const BlockGemmArgs& L, cudaStream_t stream);
 int launch_block_gemm_decode(const BlockGemmArgs& L, cudaStream_t stream);
 size_t block_gemm_decode_workspace();

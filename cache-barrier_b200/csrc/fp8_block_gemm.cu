@@ -19,7 +19,10 @@ constexpr int kBlk = 128;
 
 int launch_block_gemm(const BlockGemmArgs& L, cudaStream_t stream) {
   if (L.M <= 64) return launch_block_gemm_decode(L, stream);
-  if (block_gemm_pair_eligible(L)) return launch_block_gemm_pair(L, stream);
+  // A 256 x 256 block of a pair takes about 0.66 us, a 128 x 128 block of a CTA 0.5 us
+  // when all SMs are busy (M x N x K = 512 x 8192 x 8192: 47 us against 73 us;
+  // 256 x 8192 x 8192: 46 us against 36 us).
+  if (4 * block_gemm_pair_blocks(L) < 3 * block_gemm_tc_blocks(L)) return launch_block_gemm_pair(L, stream);
   return launch_block_gemm_tc(L, stream);
 }
 

@@ -366,10 +366,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 }  // namespace
 
-bool block_gemm_pair_eligible(const BlockGemmArgs& L) {
-  const int sms = sm_count();
+long long block_gemm_pair_blocks(const BlockGemmArgs& L) {
+  const int pairs = sm_count() / 2;
   const long long tiles = L.batch * ((L.M + 255) / 256) * ((L.N + 255) / 256);
-  return tiles >= 2LL * sms;
+  return pairs > 0 ? (tiles + pairs - 1) / pairs * ((L.K + kBK - 1) / kBK) : 0;
 }
 
 int launch_block_gemm_pair(const BlockGemmArgs& L, cudaStream_t stream) {
