@@ -48,6 +48,10 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16 * kWarps;  // tokens per tile
+constexpr int kCtasPerSm = 4;       // at most; a kernel's registers may allow fewer
+// Units that an item's set-up (query fragments, joining the warps) counts for when
+// the tiles are dealt out: with mixed lengths some CTAs hold many short items.
+constexpr int kItemCost = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -63,6 +67,7 @@ struct AttnParams {
   float* lse;  // optional
   float scale;
   int B, heads, G, blocks;  // kv heads, queries per kv head, head blocks (of 8 * NT queries) per kv head
+  int q_vec;  // query rows are 8-byte aligned
   int num_pages, page, page_shift, max_pages;  // page_shift: log2(page) or -1
   long long q_sb, q_sh, o_sb, o_sh, lse_sb, table_sb;
   long long k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;  // in bytes
@@ -166,6 +171,8 @@ struct Shape {
   // the division by their sum takes out: f16 then keeps them normal down to 2^-29
   // instead of 2^-14 (a long context's typical weight). bf16 has fp32's range.
   static constexpr float kShift = kBf16 ? 0.0f : 15.0f;
+  // bf16 queries over an e4m3 cache: rows are scaled into f16's range
+  static constexpr bool kScaleQ = FP8 && std::is_same<QT, __nv_bfloat16>::value;
   static constexpr int kElem = FP8 ? 1 : 2;
   static constexpr int kHeads = 8 * NT;          // query heads of a head block
   static constexpr int kKC = D * kElem / 64;     // 16-byte chunks of K per lane and token (four lanes share a row)
@@ -213,102 +220,54 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
     if (p.lse)
       for (int h = tid; h < p.heads * p.G; h += kThreads) p.lse[b * p.lse_sb + h] = -INFINITY;
   }
-  // This CTA's tiles [t0, t1) of the T tiles, and the sequence that holds t0.
-  long long T = 0;
-  for (int base = 0; base < p.B; base += kThreads) {
-    const int b = base + tid;
-    const long long n = b < p.B ? static_cast<long long>((length(b) + kTile - 1) / kTile) * per_b : 0;
+  // This CTA's units [t0, t1) of the T units (an item is kItemCost units of set-up,
+  // then its tiles), and the sequence that holds t0. Up to kThreads sequences one scan
+  // gives both.
+  auto tiles_of = [&](int b) {
+    const int n = b < p.B ? length(b) : 0;
+    return n > 0 ? static_cast<long long>((n + kTile - 1) / kTile + kItemCost) * per_b : 0LL;
+  };
+  long long n = tiles_of(tid), chunk, T;
+  long long incl = block_scan(n, sh_scan, &chunk);
+  T = chunk;
+  for (int base = kThreads; base < p.B; base += kThreads) {
     long long sum;
-    block_scan(n, sh_scan, &sum);
+    block_scan(tiles_of(base + tid), sh_scan, &sum);
     T += sum;
   }
   if (bad && p.status) atomicOr(p.status, CB_DEVERR_BAD_INDEX);
-  // no more CTAs than tiles take part, so every one between an item's first and last holds a part of it
+  // no more CTAs than units take part, so every one between an item's first and last tile holds a part of it
   const int grid = T < static_cast<long long>(gridDim.x) ? static_cast<int>(T) : static_cast<int>(gridDim.x);
   const int cta = static_cast<int>(blockIdx.x);
   if (cta >= grid) return;
   const long long t0 = cta * T / grid, t1 = (cta + 1) * T / grid;
-  long long before = 0;
-  for (int base = 0; base < p.B; base += kThreads) {
-    const int b = base + tid;
-    const long long n = b < p.B ? static_cast<long long>((length(b) + kTile - 1) / kTile) * per_b : 0;
-    long long sum;
-    const long long incl = block_scan(n, sh_scan, &sum) + before;
+  for (long long base = 0, before = 0;;) {
     if (t0 >= incl - n && t0 < incl) {
-      sh_found[0] = b;
+      sh_found[0] = base + tid;
       sh_found[1] = incl - n;
     }
-    before += sum;
+    before += chunk;
     if (t0 < before) break;  // uniform
+    base += kThreads;
+    n = tiles_of(static_cast<int>(base) + tid);
+    incl = block_scan(n, sh_scan, &chunk) + before;
   }
   __syncthreads();
   int b = static_cast<int>(sh_found[0]);
   int len = length(b);
   int tiles = (len + kTile - 1) / kTile;
-  int item = static_cast<int>((t0 - sh_found[1]) / tiles);         // item within the sequence
-  int tile = static_cast<int>(t0 - sh_found[1] - static_cast<long long>(item) * tiles);  // tile within the item
-  long long at = t0;
+  int item = static_cast<int>((t0 - sh_found[1]) / (tiles + kItemCost));  // item within the sequence
+  // first unit of the item, and this CTA's first tile in it (0 if the range begins in the set-up units)
+  long long item_at = sh_found[1] + static_cast<long long>(item) * (tiles + kItemCost);
+  int tile = t0 - item_at > kItemCost ? static_cast<int>(t0 - item_at) - kItemCost : 0;
 
-  while (at < t1) {
+  while (item_at + kItemCost < t1) {  // its first tile at least is in the range
+    const long long item_first = item_at + kItemCost;  // unit of the item's first tile
     const int head = item / p.blocks, blk = item - head * p.blocks;
     const int q0 = blk * S::kHeads;                                   // first query of the block, within its group
     const int nq = p.G - q0 < S::kHeads ? p.G - q0 : S::kHeads;       // queries of the block
-    const int tile_end = tiles - tile < t1 - at ? tiles : tile + static_cast<int>(t1 - at);
-    const long long item_first = at - tile;  // global index of the item's first tile
+    const int tile_end = tiles < t1 - item_first ? tiles : static_cast<int>(t1 - item_first);
     const QT* qrow = static_cast<const QT*>(p.q) + b * p.q_sb + static_cast<long long>(head * p.G + q0) * p.q_sh;
-
-    // ---- query fragments ----
-    __syncthreads();  // the previous item is done with the shared memory
-    if constexpr (FP8) {
-      // power of two that brings each query row's largest value to [1, 2)
-      for (int r = warp; r < S::kHeads; r += kWarps) {
-        float m = 0.0f;
-        if (r < nq)
-          for (int d = lane; d < D; d += 32) m = fmaxf(m, fabsf(q_val(qrow + r * p.q_sh + d)));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        int e = 0;
-        if (m > 0.0f && m < INFINITY) e = ilogbf(m);
-        if (e < -100) e = -100;  // rows below 2^-100 keep a factor that fp32 holds
-        if (lane == 0) sh_qexp[r] = ldexpf(1.0f, e);
-      }
-      __syncthreads();
-    }
-    for (int i = tid; i < S::kKSteps * NT * 32; i += kThreads) {
-      const int l = i & 31, r = (i >> 5) % NT * 8 + (l >> 2), ks = (i >> 5) / NT;
-      // d of the k-step's four elements in lane t: the order of K's 16-byte chunks
-      const int d = FP8 ? (ks >> 2) * 64 + (l & 3) * 16 + (ks & 3) * 4 : (ks >> 1) * 32 + (l & 3) * 8 + (ks & 1) * 4;
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (r < nq) {
-        const float f = FP8 ? 1.0f / sh_qexp[r] : 1.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = q_val(qrow + r * p.q_sh + d + j) * f;
-      }
-      sh_q[i] = make_uint2(M::pack(v[0], v[1]), M::pack(v[2], v[3]));
-    }
-    __syncthreads();
-    float zs[NT][2];  // score factor of this lane's two heads
-    const float ks_head = FP8 && p.k_scale ? p.k_scale[head] : 1.0f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        zs[n][j] = p.scale * kLog2e;
-        if constexpr (FP8) zs[n][j] = p.scale * ks_head * sh_qexp[n * 8 + 2 * t + j] * kLog2e;
-      }
-
-    float o[S::kKSteps][NT][4];
-    float m_run[NT][2], l_run[NT][2];
-#pragma unroll
-    for (int i = 0; i < S::kKSteps; ++i)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][n][j] = 0.0f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) m_run[n][j] = -INFINITY, l_run[n][j] = 0.0f;
 
     const int* trow = p.table + b * p.table_sb;
     const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + head * p.k_sh;
@@ -325,26 +284,30 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
       return pg;
     };
 
-    for (int tl = tile; tl < tile_end; ++tl) {
+    // K and V of tile tl for this warp: 16 tokens, rows past the length zero
+    uint4 kr[2][S::kKC];
+    uint4 vr[4][S::kVC];
+    bool k_ok[2];
+    int my_pg = -1;  // page of this lane's token (lane & 15); with PAGE16 all 16 share one page
+    auto find_page = [&](int tl) {
       const int tok0 = tl * kTile + warp * 16;
-      if (tok0 >= len) break;  // the item's last tile: no token for this warp
-      // page of this lane's token (lane & 15); with PAGE16 all 16 share one page
-      const int my_pg = lookup(PAGE16 ? tok0 : tok0 + (lane & 15));
-      uint4 kr[2][S::kKC];
-      uint4 vr[4][S::kVC];
-      bool k_ok[2];
+      my_pg = lookup(PAGE16 ? tok0 : tok0 + (lane & 15));
+    };
+    auto load_k = [&](int tl) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int rel = g + 8 * r, tok = tok0 + rel;
+        const int rel = g + 8 * r, tok = tl * kTile + warp * 16 + rel;
         const int pg = PAGE16 ? my_pg : __shfl_sync(0xffffffffu, my_pg, rel);
         k_ok[r] = tok < len && pg >= 0;
         const uint8_t* row = kbase + pg * p.k_sp + static_cast<long long>(tok - page_of(tok) * p.page) * p.k_ss + t * 16;
 #pragma unroll
         for (int c = 0; c < S::kKC; ++c) kr[r][c] = k_ok[r] ? ldg16(row + c * 64) : make_uint4(0, 0, 0, 0);
       }
+    };
+    auto load_v = [&](int tl) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int rel = 2 * t + (r & 1) + 8 * (r >> 1), tok = tok0 + rel;
+        const int rel = 2 * t + (r & 1) + 8 * (r >> 1), tok = tl * kTile + warp * 16 + rel;
         const int pg = PAGE16 ? my_pg : __shfl_sync(0xffffffffu, my_pg, rel);
         const bool ok = tok < len && pg >= 0;
         const uint8_t* row =
@@ -359,6 +322,94 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
           }
         }
       }
+    };
+    // this warp's tiles: its 16 tokens of the item's last tile may lie past the length
+    const int w_end = (tile_end - 1) * kTile + warp * 16 < len ? tile_end : tile_end - 1;
+    // the first tile's loads cover the query's
+    if (tile < w_end) {
+      find_page(tile);
+      load_k(tile);
+      load_v(tile);
+    }
+
+    // ---- query fragments ----
+    __syncthreads();  // the previous item is done with the shared memory
+    // four consecutive elements of a query row
+    auto q4 = [&](int r, int d, float (&v)[4]) {
+      const QT* src = qrow + r * p.q_sh + d;
+      if (p.q_vec) {
+        const uint2 raw = *reinterpret_cast<const uint2*>(src);
+        const QT* e = reinterpret_cast<const QT*>(&raw);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = q_val(e + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = q_val(src + j);
+      }
+    };
+    if constexpr (S::kScaleQ) {
+      // power of two that brings each query row's largest value to [1, 2)
+      for (int r = warp; r < S::kHeads; r += kWarps) {
+        float m = 0.0f;
+        if (r < nq) {
+          for (int d = lane * 4; d < D; d += 128) {
+            float v[4];
+            q4(r, d, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[j]));
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        int e = 0;
+        if (m > 0.0f && m < INFINITY) e = ilogbf(m);
+        if (e < -100) e = -100;  // rows below 2^-100 keep a factor that fp32 holds
+        if (lane == 0) sh_qexp[r] = ldexpf(1.0f, e);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < S::kKSteps * NT * 32 / kThreads; ++x) {
+      const int i = x * kThreads + tid;
+      const int l = i & 31, r = (i >> 5) % NT * 8 + (l >> 2), ks = (i >> 5) / NT;
+      // d of the k-step's four elements in lane t: the order of K's 16-byte chunks
+      const int d = FP8 ? (ks >> 2) * 64 + (l & 3) * 16 + (ks & 3) * 4 : (ks >> 1) * 32 + (l & 3) * 8 + (ks & 1) * 4;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < nq) {
+        q4(r, d, v);
+        if constexpr (S::kScaleQ) {
+          const float f = 1.0f / sh_qexp[r];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] *= f;
+        }
+      }
+      sh_q[i] = make_uint2(M::pack(v[0], v[1]), M::pack(v[2], v[3]));
+    }
+    __syncthreads();
+    float zs[NT][2];  // score factor of this lane's two heads
+    const float ks_head = FP8 && p.k_scale ? p.k_scale[head] : 1.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        zs[n][j] = p.scale * kLog2e;
+        if constexpr (FP8) zs[n][j] = p.scale * ks_head * kLog2e * (S::kScaleQ ? sh_qexp[n * 8 + 2 * t + j] : 1.0f);
+      }
+
+    float o[S::kKSteps][NT][4];
+    float m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int i = 0; i < S::kKSteps; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][n][j] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) m_run[n][j] = -INFINITY, l_run[n][j] = 0.0f;
+
+    for (int tl = tile; tl < w_end; ++tl) {
       // ---- scores ----
       float s[NT][4];
 #pragma unroll
@@ -385,13 +436,18 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
           }
         }
       }
+      const bool ok[2] = {k_ok[0], k_ok[1]};
+      if (tl + 1 < w_end) {
+        find_page(tl + 1);
+        load_k(tl + 1);
+      }
       // ---- running maximum and sum ----
       uint32_t pb[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float x[4], mx[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = k_ok[j >> 1] ? s[n][j] * zs[n][j & 1] : -INFINITY;
+        for (int j = 0; j < 4; ++j) x[j] = ok[j >> 1] ? s[n][j] * zs[n][j & 1] : -INFINITY;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           mx[j] = fmaxf(x[j], x[2 + j]);
@@ -445,6 +501,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
           }
         }
       }
+      if (tl + 1 < w_end) load_v(tl + 1);
     }
 
     // ---- join the warps ----
@@ -475,30 +532,6 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
     QT* orow = static_cast<QT*>(p.out) + b * p.o_sb + static_cast<long long>(head * p.G + q0) * p.o_sh;
     float* lrow = p.lse ? p.lse + b * p.lse_sb + head * p.G + q0 : nullptr;
     const float vs = FP8 && p.v_scale ? p.v_scale[head] : 1.0f;
-    // parts a .. z - 1 at `parts` (stride kPart, or by contributor), joined in order
-    auto join = [&](auto&& part_of, int n_parts, bool finish, float* dst) {
-      for (int i = tid; i < nq * D; i += kThreads) {
-        const int r = i / D, d = i - r * D;
-        float mx = -INFINITY;
-        for (int w = 0; w < n_parts; ++w) mx = fmaxf(mx, __ldcg(part_of(w) + r));
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        float sum = 0.0f, acc = 0.0f;
-        for (int w = 0; w < n_parts; ++w) {
-          const float* pt = part_of(w);
-          const float f = exp2_approx(__ldcg(pt + r) - ref);
-          sum = fmaf(f, __ldcg(pt + S::kHeads + r), sum);
-          acc = fmaf(f, __ldcg(pt + 2 * S::kHeads + r * D + d), acc);
-        }
-        if (finish) {
-          put(orow + r * p.o_sh + d, sum == 0.0f ? 0.0f : acc / sum * vs);
-          if (lrow && d == 0) lrow[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum) - S::kShift) * kLn2;
-        } else {
-          dst[2 * S::kHeads + r * D + d] = acc;
-          if (d == 0) dst[r] = mx, dst[S::kHeads + r] = sum;
-        }
-      }
-    };
-    // (generic loads: the warps' parts are in shared memory)
     auto join_warps = [&](bool finish, float* dst) {
       for (int i = tid; i < nq * D; i += kThreads) {
         const int r = i / D, d = i - r * D;
@@ -523,6 +556,66 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
         }
       }
     };
+    // A cut item's parts, joined in CTA order, kJoin at a time: their maxima and sums
+    // go to shared memory in one round trip; each thread adds its float4s of the output
+    // with the loads of four parts in flight, against a running maximum per head.
+    auto join_parts = [&](auto&& part_of, int n_parts) {
+      constexpr int kJoin = 32;
+      float* const sh_m = sh_part;                          // [kJoin][kHeads]
+      float* const sh_l = sh_part + kJoin * S::kHeads;      // [kJoin][kHeads]
+      static_assert(2 * kJoin * S::kHeads <= kWarps * S::kPart, "maxima and sums must fit");
+      constexpr int kF4 = (S::kHeads * D / 4 + kThreads - 1) / kThreads;  // float4s of a thread
+      float4 acc[kF4];
+      float mx[kF4], sum[kF4];
+#pragma unroll
+      for (int x = 0; x < kF4; ++x) acc[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), mx[x] = -INFINITY, sum[x] = 0.0f;
+      for (int w0 = 0; w0 < n_parts; w0 += kJoin) {
+        const int here = n_parts - w0 < kJoin ? n_parts - w0 : kJoin;
+        __syncthreads();
+        for (int i = tid; i < here * S::kHeads; i += kThreads) {
+          const float* pt = part_of(w0 + i / S::kHeads) + i % S::kHeads;
+          sh_m[i] = __ldcg(pt);
+          sh_l[i] = __ldcg(pt + S::kHeads);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kF4; ++x) {
+          const int e = (x * kThreads + tid) * 4, r = e / D;
+          if (r >= nq) break;
+          float top = mx[x];
+          for (int w = 0; w < here; ++w) top = fmaxf(top, sh_m[w * S::kHeads + r]);
+          const float ref = top == -INFINITY ? 0.0f : top;
+          const float f0 = exp2_approx(mx[x] - ref);
+          acc[x].x *= f0, acc[x].y *= f0, acc[x].z *= f0, acc[x].w *= f0, sum[x] *= f0;
+          mx[x] = top;
+          for (int w = 0; w < here; w += 4) {
+            float4 v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              v[y] = w + y < here ? __ldcg(reinterpret_cast<const float4*>(part_of(w0 + w + y) + 2 * S::kHeads + e))
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              if (w + y >= here) break;
+              const float f = exp2_approx(sh_m[(w + y) * S::kHeads + r] - ref);
+              sum[x] = fmaf(f, sh_l[(w + y) * S::kHeads + r], sum[x]);
+              acc[x].x = fmaf(f, v[y].x, acc[x].x), acc[x].y = fmaf(f, v[y].y, acc[x].y);
+              acc[x].z = fmaf(f, v[y].z, acc[x].z), acc[x].w = fmaf(f, v[y].w, acc[x].w);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kF4; ++x) {
+        const int e = (x * kThreads + tid) * 4, r = e / D, d = e % D;
+        if (r >= nq) break;
+        const float f = sum[x] == 0.0f ? 0.0f : vs / sum[x];
+        const float v[4] = {acc[x].x, acc[x].y, acc[x].z, acc[x].w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) put(orow + r * p.o_sh + d + y, sum[x] == 0.0f ? 0.0f : v[y] * f);
+        if (lrow && d == 0) lrow[r] = sum[x] == 0.0f ? -INFINITY : (mx[x] + log2f(sum[x]) - S::kShift) * kLn2;
+      }
+    };
     if (whole) {
       join_warps(true, nullptr);
     } else {
@@ -533,23 +626,25 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
       // slot 0: the item began in an earlier CTA (this CTA's first segment); 1: it begins here
       auto slot = [&](int c) { return p.partials + (static_cast<long long>(c) * 2 + (c == c_first ? 1 : 0)) * S::kPart; };
       join_warps(false, slot(cta));
-      __threadfence();
       __syncthreads();
-      if (tid == 0) sh_last = atomicAdd(&p.counters[c_first], 1) == c_last - c_first;
+      if (tid == 0) {
+        __threadfence();  // covers the CTA's stores before the barrier
+        sh_last = atomicAdd(&p.counters[c_first], 1) == c_last - c_first;
+      }
       __syncthreads();
       if (sh_last) {
         __threadfence();
-        join([&](int w) { return slot(c_first + w); }, c_last - c_first + 1, true, nullptr);
+        join_parts([&](int w) { return slot(c_first + w); }, c_last - c_first + 1);
         if (tid == 0) p.counters[c_first] = 0;  // the next launch starts from zero
       }
     }
 
     // ---- next item ----
-    at += tile_end - tile;
+    item_at = item_first + tiles;
     tile = 0;
     if (++item == per_b) {
       item = 0;
-      if (at < t1) {
+      if (item_at < t1) {
         do {
           ++b;
           len = length(b);
@@ -561,19 +656,26 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
 }
 
 template <typename QT, bool FP8, int D, int NT, bool PAGE16>
-int launch_kernel(const AttnParams& p, int grid, cudaStream_t stream) {
+int launch_kernel(const AttnParams& p, long long most, cudaStream_t stream) {
   using S = Shape<QT, FP8, D, NT>;
   auto kernel = attn_kernel<QT, FP8, D, NT, PAGE16>;
-  static thread_local int configured_dev = -1;
+  static thread_local int configured_dev = -1, per_sm = 1;
   int dev = 0;
   cudaGetDevice(&dev);
   if (configured_dev != dev) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, S::kSmem) != cudaSuccess)
       return CB_ERR_CUDA;
+    if (per_sm < 1) per_sm = 1;
+    if (per_sm > kCtasPerSm) per_sm = kCtasPerSm;
     configured_dev = dev;
   }
+  // every SM's share of CTAs, but no more than there can be units of work
+  long long grid = static_cast<long long>(sm_count()) * per_sm;
+  if (grid > kMaxGrid) grid = kMaxGrid;
+  if (grid > most) grid = most < 1 ? 1 : most;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
@@ -585,7 +687,6 @@ int launch_kernel(const AttnParams& p, int grid, cudaStream_t stream) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
-constexpr int kCtasPerSm = 3;
 
 int attn_grid_limit() {
   int sms = sm_count();
@@ -599,19 +700,19 @@ int attn_grid_limit() {
 int head_tiles(int G, int D) { return G > 8 && D <= 128 ? 2 : 1; }
 
 template <typename QT, bool FP8, int D>
-int dispatch_nt(const AttnParams& p, int nt, bool page16, int grid, cudaStream_t s) {
+int dispatch_nt(const AttnParams& p, int nt, bool page16, long long most, cudaStream_t s) {
   if constexpr (D <= 128) {
     if (nt == 2)
-      return page16 ? launch_kernel<QT, FP8, D, 2, true>(p, grid, s) : launch_kernel<QT, FP8, D, 2, false>(p, grid, s);
+      return page16 ? launch_kernel<QT, FP8, D, 2, true>(p, most, s) : launch_kernel<QT, FP8, D, 2, false>(p, most, s);
   }
-  return page16 ? launch_kernel<QT, FP8, D, 1, true>(p, grid, s) : launch_kernel<QT, FP8, D, 1, false>(p, grid, s);
+  return page16 ? launch_kernel<QT, FP8, D, 1, true>(p, most, s) : launch_kernel<QT, FP8, D, 1, false>(p, most, s);
 }
 
 template <typename QT, bool FP8>
-int dispatch_d(const AttnParams& p, int D, int nt, bool page16, int grid, cudaStream_t s) {
-  if (D == 64) return dispatch_nt<QT, FP8, 64>(p, nt, page16, grid, s);
-  if (D == 128) return dispatch_nt<QT, FP8, 128>(p, nt, page16, grid, s);
-  return dispatch_nt<QT, FP8, 256>(p, nt, page16, grid, s);
+int dispatch_d(const AttnParams& p, int D, int nt, bool page16, long long most, cudaStream_t s) {
+  if (D == 64) return dispatch_nt<QT, FP8, 64>(p, nt, page16, most, s);
+  if (D == 128) return dispatch_nt<QT, FP8, 128>(p, nt, page16, most, s);
+  return dispatch_nt<QT, FP8, 256>(p, nt, page16, most, s);
 }
 
 size_t part_bytes(int G, int D) {
@@ -666,6 +767,7 @@ extern "C" CB_API int cb_paged_decode_attention(const void* q, int q_dtype, cons
   p.blocks = (G + 8 * nt - 1) / (8 * nt);
   p.num_pages = static_cast<int>(num_pages), p.page = static_cast<int>(page_size);
   p.max_pages = static_cast<int>(max_pages);
+  p.q_vec = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && strides[0] % 4 == 0 && strides[1] % 4 == 0;
   p.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (page_size == (1LL << s)) p.page_shift = s;
@@ -673,20 +775,17 @@ extern "C" CB_API int cb_paged_decode_attention(const void* q, int q_dtype, cons
   p.lse_sb = strides[4], p.table_sb = strides[5];
   p.k_sp = strides[6] * e, p.k_ss = strides[7] * e, p.k_sh = strides[8] * e;
   p.v_sp = strides[9] * e, p.v_ss = strides[10] * e, p.v_sh = strides[11] * e;
-  // Grid: every SM's share of CTAs, but no more than there can be tiles.
   const long long cap = max_pages * page_size;
-  const long long most = B * Hkv * p.blocks * ((cap + kTile - 1) / kTile);
-  long long grid = attn_grid_limit();
-  if (grid > most) grid = most < 1 ? 1 : most;
+  const long long most = B * Hkv * p.blocks * ((cap + kTile - 1) / kTile + kItemCost);
   const size_t need = workspace_need(attn_grid_limit(), part_bytes(G, static_cast<int>(D)));
   if (!workspace || workspace_bytes < need) return CB_ERR_WORKSPACE;
-  Workspace ws = carve_workspace(workspace, static_cast<int>(grid));
+  Workspace ws = carve_workspace(workspace, attn_grid_limit());
   p.status = ws.status, p.counters = ws.counters, p.partials = static_cast<float*>(ws.partials);
   const bool page16 = page_size % 16 == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (q_dtype == CB_DTYPE_BF16)
-    return fp8 ? dispatch_d<__nv_bfloat16, true>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s)
-               : dispatch_d<__nv_bfloat16, false>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s);
-  return fp8 ? dispatch_d<__half, true>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s)
-             : dispatch_d<__half, false>(p, static_cast<int>(D), nt, page16, static_cast<int>(grid), s);
+    return fp8 ? dispatch_d<__nv_bfloat16, true>(p, static_cast<int>(D), nt, page16, most, s)
+               : dispatch_d<__nv_bfloat16, false>(p, static_cast<int>(D), nt, page16, most, s);
+  return fp8 ? dispatch_d<__half, true>(p, static_cast<int>(D), nt, page16, most, s)
+             : dispatch_d<__half, false>(p, static_cast<int>(D), nt, page16, most, s);
 }
