@@ -52,6 +52,9 @@ constexpr int kCtasPerSm = 4;       // at most; a kernel's registers may allow f
 // Units that an item's set-up (query fragments, joining the warps) counts for when
 // the tiles are dealt out: with mixed lengths some CTAs hold many short items.
 constexpr int kItemCost = 2;
+constexpr int kWholeTiles = 4;     // items up to this are not cut
+constexpr int kJoinThreads = 256;  // of join_kernel
+constexpr int kPartsApart = 20;    // parts per item from which they are joined in a launch of their own
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -71,6 +74,8 @@ struct AttnParams {
   int num_pages, page, page_shift, max_pages;  // page_shift: log2(page) or -1
   long long q_sb, q_sh, o_sb, o_sh, lse_sb, table_sb;
   long long k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;  // in bytes
+  int grid;        // CTAs launched
+  int join_apart;  // cut items are joined by join_kernel
   int* status;
   int* counters;
   float* partials;
@@ -257,16 +262,32 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
   int len = length(b);
   int tiles = (len + kTile - 1) / kTile;
   int item = static_cast<int>((t0 - sh_found[1]) / (tiles + kItemCost));  // item within the sequence
-  // first unit of the item, and this CTA's first tile in it (0 if the range begins in the set-up units)
-  long long item_at = sh_found[1] + static_cast<long long>(item) * (tiles + kItemCost);
+  long long item_at = sh_found[1] + static_cast<long long>(item) * (tiles + kItemCost);  // first unit of the item
+  auto next_item = [&] {
+    item_at += tiles + kItemCost;
+    if (++item == per_b) {
+      item = 0;
+      if (item_at < t1) {
+        do {
+          ++b;
+          len = length(b);
+        } while (len == 0);
+        tiles = (len + kTile - 1) / kTile;
+      }
+    }
+  };
+  // A short item belongs as a whole to the CTA that holds its first unit.
+  if (tiles <= kWholeTiles && t0 > item_at) next_item();
+  // this CTA's first tile in the item (0 if the range begins in the set-up units)
   int tile = t0 - item_at > kItemCost ? static_cast<int>(t0 - item_at) - kItemCost : 0;
 
-  while (item_at + kItemCost < t1) {  // its first tile at least is in the range
+  for (; item_at + (tiles <= kWholeTiles ? 0 : kItemCost) < t1; next_item(), tile = 0) {
     const long long item_first = item_at + kItemCost;  // unit of the item's first tile
     const int head = item / p.blocks, blk = item - head * p.blocks;
     const int q0 = blk * S::kHeads;                                   // first query of the block, within its group
     const int nq = p.G - q0 < S::kHeads ? p.G - q0 : S::kHeads;       // queries of the block
-    const int tile_end = tiles < t1 - item_first ? tiles : static_cast<int>(t1 - item_first);
+    const int tile_end =
+        tiles <= kWholeTiles || tiles < t1 - item_first ? tiles : static_cast<int>(t1 - item_first);
     const QT* qrow = static_cast<const QT*>(p.q) + b * p.q_sb + static_cast<long long>(head * p.G + q0) * p.q_sh;
 
     const int* trow = p.table + b * p.table_sb;
@@ -578,29 +599,38 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
           sh_l[i] = __ldcg(pt + S::kHeads);
         }
         __syncthreads();
+        float ref[kF4];
 #pragma unroll
         for (int x = 0; x < kF4; ++x) {
-          const int e = (x * kThreads + tid) * 4, r = e / D;
-          if (r >= nq) break;
+          const int r = (x * kThreads + tid) * 4 / D;
           float top = mx[x];
           for (int w = 0; w < here; ++w) top = fmaxf(top, sh_m[w * S::kHeads + r]);
-          const float ref = top == -INFINITY ? 0.0f : top;
-          const float f0 = exp2_approx(mx[x] - ref);
+          ref[x] = top == -INFINITY ? 0.0f : top;
+          const float f0 = exp2_approx(mx[x] - ref[x]);
           acc[x].x *= f0, acc[x].y *= f0, acc[x].z *= f0, acc[x].w *= f0, sum[x] *= f0;
           mx[x] = top;
-          for (int w = 0; w < here; w += 4) {
-            float4 v[4];
+        }
+        for (int w = 0; w < here; w += 4) {
+          float4 v[4][kF4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-              v[y] = w + y < here ? __ldcg(reinterpret_cast<const float4*>(part_of(w0 + w + y) + 2 * S::kHeads + e))
-                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int y = 0; y < 4; ++y)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              if (w + y >= here) break;
-              const float f = exp2_approx(sh_m[(w + y) * S::kHeads + r] - ref);
+            for (int x = 0; x < kF4; ++x) {
+              const int e = (x * kThreads + tid) * 4;
+              v[y][x] = w + y < here && e < nq * D
+                            ? __ldcg(reinterpret_cast<const float4*>(part_of(w0 + w + y) + 2 * S::kHeads + e))
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            if (w + y >= here) break;
+#pragma unroll
+            for (int x = 0; x < kF4; ++x) {
+              const int r = (x * kThreads + tid) * 4 / D;
+              const float f = exp2_approx(sh_m[(w + y) * S::kHeads + r] - ref[x]);
               sum[x] = fmaf(f, sh_l[(w + y) * S::kHeads + r], sum[x]);
-              acc[x].x = fmaf(f, v[y].x, acc[x].x), acc[x].y = fmaf(f, v[y].y, acc[x].y);
-              acc[x].z = fmaf(f, v[y].z, acc[x].z), acc[x].w = fmaf(f, v[y].w, acc[x].w);
+              acc[x].x = fmaf(f, v[y][x].x, acc[x].x), acc[x].y = fmaf(f, v[y][x].y, acc[x].y);
+              acc[x].z = fmaf(f, v[y][x].z, acc[x].z), acc[x].w = fmaf(f, v[y][x].w, acc[x].w);
             }
           }
         }
@@ -626,6 +656,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
       // slot 0: the item began in an earlier CTA (this CTA's first segment); 1: it begins here
       auto slot = [&](int c) { return p.partials + (static_cast<long long>(c) * 2 + (c == c_first ? 1 : 0)) * S::kPart; };
       join_warps(false, slot(cta));
+      if (p.join_apart) continue;  // join_kernel follows
       __syncthreads();
       if (tid == 0) {
         __threadfence();  // covers the CTA's stores before the barrier
@@ -638,25 +669,108 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
         if (tid == 0) p.counters[c_first] = 0;  // the next launch starts from zero
       }
     }
-
-    // ---- next item ----
-    item_at = item_first + tiles;
-    tile = 0;
-    if (++item == per_b) {
-      item = 0;
-      if (item_at < t1) {
-        do {
-          ++b;
-          len = length(b);
-        } while (len == 0);
-        tiles = (len + kTile - 1) / kTile;
-      }
-    }
   }
 }
 
+// Joins the parts of cut items in a launch of its own, where few items have many parts
+// each (one CTA would read them all): a CTA per item and head, D / 4 threads per part.
+template <typename QT, bool FP8, int D, int NT>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p) {
+  using S = Shape<QT, FP8, D, NT>;
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAhead = 8;
+  __shared__ float sh_m[kGroups], sh_l[kGroups];
+  __shared__ float4 sh_v[kGroups][kLanes];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int per_b = p.heads * p.blocks;
+  const int b = blockIdx.x / per_b, item = blockIdx.x - b * per_b;
+  const int head = item / p.blocks, q0 = (item - head * p.blocks) * S::kHeads, r = blockIdx.y;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (q0 + r >= p.G) return;
+  // the same dealing out as the kernel before (B <= 32: every lane one sequence)
+  const long long cap = static_cast<long long>(p.max_pages) * p.page;
+  long long units = 0, mine = 0;
+  int tiles = 0;
+  if (lane < p.B) {
+    const int n = p.lens[lane];
+    const long long len = n < 0 ? 0 : n > cap ? cap : n;
+    tiles = static_cast<int>((len + kTile - 1) / kTile);
+    units = tiles > 0 ? static_cast<long long>(tiles + kItemCost) * per_b : 0;
+    mine = lane < b ? units : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    units += __shfl_xor_sync(0xffffffffu, units, o);
+    mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  }
+  tiles = __shfl_sync(0xffffffffu, tiles, b);
+  if (tiles <= kWholeTiles) return;
+  const long long T = units, grid = T < p.grid ? T : p.grid;
+  const long long first = mine + static_cast<long long>(item) * (tiles + kItemCost) + kItemCost;
+  const int c_first = static_cast<int>(((first + 1) * grid - 1) / T);
+  const int n_parts = static_cast<int>(((first + tiles) * grid - 1) / T) - c_first + 1;
+  if (n_parts == 1) return;  // stored by its CTA
+  auto part_of = [&](int w) { return p.partials + (static_cast<long long>(c_first + w) * 2 + (w == 0 ? 1 : 0)) * S::kPart; };
+
+  const int group = tid / kLanes, e = tid % kLanes;
+  float mx = -INFINITY, sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int w0 = group; w0 < n_parts; w0 += kGroups * kAhead) {
+    float m[kAhead], l[kAhead];
+    float4 v[kAhead];
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      const bool in = w0 + y * kGroups < n_parts;
+      const float* pt = part_of(in ? w0 + y * kGroups : w0);
+      m[y] = in ? __ldcg(pt + r) : -INFINITY;
+      l[y] = in ? __ldcg(pt + S::kHeads + r) : 0.0f;
+      v[y] = __ldcg(reinterpret_cast<const float4*>(pt + 2 * S::kHeads + r * D) + e);
+    }
+    float top = mx;
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) top = fmaxf(top, m[y]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float f0 = exp2_approx(mx - ref);
+    mx = top;
+    acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0, sum *= f0;
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      if (w0 + y * kGroups >= n_parts) break;
+      const float f = exp2_approx(m[y] - ref);
+      sum = fmaf(f, l[y], sum);
+      acc.x = fmaf(f, v[y].x, acc.x), acc.y = fmaf(f, v[y].y, acc.y);
+      acc.z = fmaf(f, v[y].z, acc.z), acc.w = fmaf(f, v[y].w, acc.w);
+    }
+  }
+  sh_v[group][e] = acc;
+  if (e == 0) sh_m[group] = mx, sh_l[group] = sum;
+  __syncthreads();
+  if (group != 0) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kGroups; ++w) top = fmaxf(top, sh_m[w]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kGroups; ++w) {
+    const float f = exp2_approx(sh_m[w] - ref);
+    const float4 u = sh_v[w][e];
+    sum = fmaf(f, sh_l[w], sum);
+    acc.x = fmaf(f, u.x, acc.x), acc.y = fmaf(f, u.y, acc.y), acc.z = fmaf(f, u.z, acc.z), acc.w = fmaf(f, u.w, acc.w);
+  }
+  const int hq = head * p.G + q0 + r;
+  const float vs = FP8 && p.v_scale ? p.v_scale[head] : 1.0f;
+  const float f = sum == 0.0f ? 0.0f : vs / sum;
+  const float o[4] = {acc.x, acc.y, acc.z, acc.w};
+  QT* out = static_cast<QT*>(p.out) + b * p.o_sb + static_cast<long long>(hq) * p.o_sh + e * 4;
+#pragma unroll
+  for (int y = 0; y < 4; ++y) put(out + y, sum == 0.0f ? 0.0f : o[y] * f);
+  if (p.lse && e == 0) p.lse[b * p.lse_sb + hq] = sum == 0.0f ? -INFINITY : (top + log2f(sum) - S::kShift) * kLn2;
+}
+
 template <typename QT, bool FP8, int D, int NT, bool PAGE16>
-int launch_kernel(const AttnParams& p, long long most, cudaStream_t stream) {
+int launch_kernel(AttnParams p, long long most, cudaStream_t stream) {
   using S = Shape<QT, FP8, D, NT>;
   auto kernel = attn_kernel<QT, FP8, D, NT, PAGE16>;
   static thread_local int configured_dev = -1, per_sm = 1;
@@ -674,6 +788,9 @@ int launch_kernel(const AttnParams& p, long long most, cudaStream_t stream) {
   long long grid = static_cast<long long>(sm_count()) * per_sm;
   if (grid > kMaxGrid) grid = kMaxGrid;
   if (grid > most) grid = most < 1 ? 1 : most;
+  const long long items = static_cast<long long>(p.B) * p.heads * p.blocks;
+  p.grid = static_cast<int>(grid);
+  p.join_apart = p.B <= 32 && grid >= items * kPartsApart;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kThreads);
@@ -684,7 +801,12 @@ int launch_kernel(const AttnParams& p, long long most, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess || !p.join_apart) return cuda_status(e);
+  cfg.gridDim = dim3(static_cast<unsigned>(items), p.G < S::kHeads ? p.G : S::kHeads);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, join_kernel<QT, FP8, D, NT>, p));
 }
 
 

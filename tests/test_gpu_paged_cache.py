@@ -137,7 +137,8 @@ def test_pages_and_layouts(cuda_device, page, dtype, cache_dtype, layout):
     assert ops.device_status(cuda_device) == 0
 
 
-@pytest.mark.parametrize("lens", [[1], [0], [0, 0, 0], [64] * 7, [4097], [1] * 300, list(range(260)), [9000, 1, 1, 0, 700]])
+@pytest.mark.parametrize("lens", [[1], [0], [0, 0, 0], [64] * 7, [4097], [1] * 300, list(range(260)), [9000, 1, 1, 0, 700], [40000],
+                                  [257, 256, 255, 320, 321] * 9])
 @pytest.mark.parametrize("dtype,cache_dtype", [TYPES[0], TYPES[3]])
 def test_lengths(cuda_device, lens, dtype, cache_dtype):
     from cb200 import ops
