@@ -148,6 +148,38 @@ __device__ __forceinline__ float q_val(const __nv_bfloat16* p) { return __bfloat
 __device__ __forceinline__ void put(__half* o, float v) { *o = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* o, float v) { *o = __float2bfloat16_rn(v); }
 
+// The T units of all items dealt to `grid` CTAs: CTA c holds units [start(c), start(c + 1)),
+// start(c) = floor(c * T / grid). 32-bit divisions where T allows.
+struct Deal {
+  long long T, q;
+  int grid;
+  unsigned r;
+  __device__ __forceinline__ Deal(long long units, int max_grid) : T(units) {
+    // no more CTAs than units take part, so every one between an item's first and last
+    // tile holds a part of it
+    grid = T < max_grid ? static_cast<int>(T) : max_grid;
+    if (T < (1LL << 31)) {
+      const unsigned t = static_cast<unsigned>(T), n = grid > 0 ? static_cast<unsigned>(grid) : 1u;
+      q = t / n;
+      r = t - static_cast<unsigned>(q) * n;
+    } else {
+      q = T / grid;
+      r = static_cast<unsigned>(T - q * grid);
+    }
+  }
+  __device__ __forceinline__ long long start(int c) const {
+    return c * q + static_cast<unsigned>(c) * r / static_cast<unsigned>(grid);  // c * r < 2^20
+  }
+  // CTA that holds unit u: a guess in floating point, then exact.
+  __device__ __forceinline__ int owner(long long u) const {
+    int c = static_cast<int>((static_cast<float>(u) + 0.5f) * static_cast<float>(grid) / static_cast<float>(T));
+    if (c >= grid) c = grid - 1;
+    while (start(c) > u) --c;
+    while (start(c + 1) <= u) ++c;
+    return c;
+  }
+};
+
 // Inclusive sum over the CTA's threads; *total receives the whole sum.
 __device__ __forceinline__ long long block_scan(long long v, long long* sh, long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -185,21 +217,26 @@ struct Shape {
   static constexpr int kVV = kVLane >= 16 ? 16 : 8;  // bytes of one load
   static constexpr int kVC = kVLane / kVV;
   static constexpr int kKSteps = D / 16;
+  // CTAs per SM that the registers are to leave room for
+  static constexpr int kMinCtas = D == 64 ? 4 : NT == 1 && (D == 128 || FP8) ? 3 : 2;
   // part of a cut item: max and sum per head, output per head and d
   static constexpr int kPart = kHeads * 2 + kHeads * D;
-  static constexpr size_t kSmem = sizeof(float) * kWarps * kPart + sizeof(uint2) * kKSteps * NT * 32;
+  // a warp's part in shared memory: rows padded so that the fragments' stores spread over the banks
+  static constexpr int kPitch = D + 1;
+  static constexpr int kPartSh = kHeads * 2 + kHeads * kPitch;
+  static constexpr size_t kSmem = sizeof(float) * kWarps * kPartSh + sizeof(uint2) * kKSteps * NT * 32;
 };
 
 template <typename QT, bool FP8, int D, int NT, bool PAGE16>
-__global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, Shape<QT, FP8, D, NT>::kMinCtas) attn_kernel(const AttnParams p) {
   using S = Shape<QT, FP8, D, NT>;
   using M = Math<S::kBf16>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  float* const sh_part = reinterpret_cast<float*>(smem_raw);  // [warp][kPart]
-  uint2* const sh_q = reinterpret_cast<uint2*>(sh_part + kWarps * S::kPart);  // query fragments [k-step][NT][lane]
+  float* const sh_part = reinterpret_cast<float*>(smem_raw);  // [warp][kPartSh]
+  uint2* const sh_q = reinterpret_cast<uint2*>(sh_part + kWarps * S::kPartSh);  // query fragments [k-step][NT][lane]
   __shared__ long long sh_scan[kWarps];
-  __shared__ long long sh_found[2];
-  __shared__ float sh_qexp[S::kHeads];
+  __shared__ long long sh_found[3];
+  __shared__ float sh_qexp[S::kHeads], sh_qmax[kWarps][8];
   __shared__ int sh_last;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -241,15 +278,15 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
     T += sum;
   }
   if (bad && p.status) atomicOr(p.status, CB_DEVERR_BAD_INDEX);
-  // no more CTAs than units take part, so every one between an item's first and last tile holds a part of it
-  const int grid = T < static_cast<long long>(gridDim.x) ? static_cast<int>(T) : static_cast<int>(gridDim.x);
+  const Deal deal(T, static_cast<int>(gridDim.x));
   const int cta = static_cast<int>(blockIdx.x);
-  if (cta >= grid) return;
-  const long long t0 = cta * T / grid, t1 = (cta + 1) * T / grid;
+  if (cta >= deal.grid) return;
+  const long long t0 = deal.start(cta), t1 = deal.start(cta + 1);
   for (long long base = 0, before = 0;;) {
     if (t0 >= incl - n && t0 < incl) {
       sh_found[0] = base + tid;
       sh_found[1] = incl - n;
+      sh_found[2] = length(static_cast<int>(base) + tid);
     }
     before += chunk;
     if (t0 < before) break;  // uniform
@@ -259,9 +296,11 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
   }
   __syncthreads();
   int b = static_cast<int>(sh_found[0]);
-  int len = length(b);
+  int len = static_cast<int>(sh_found[2]);
   int tiles = (len + kTile - 1) / kTile;
-  int item = static_cast<int>((t0 - sh_found[1]) / (tiles + kItemCost));  // item within the sequence
+  const long long in_b = t0 - sh_found[1];
+  int item = in_b < (1LL << 31) ? static_cast<int>(static_cast<unsigned>(in_b) / static_cast<unsigned>(tiles + kItemCost))
+                                : static_cast<int>(in_b / (tiles + kItemCost));  // item within the sequence
   long long item_at = sh_found[1] + static_cast<long long>(item) * (tiles + kItemCost);  // first unit of the item
   auto next_item = [&] {
     item_at += tiles + kItemCost;
@@ -346,65 +385,68 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
     };
     // this warp's tiles: its 16 tokens of the item's last tile may lie past the length
     const int w_end = (tile_end - 1) * kTile + warp * 16 < len ? tile_end : tile_end - 1;
-    // the first tile's loads cover the query's
+    // Query fragments: four consecutive elements for each of this thread's k-steps, all
+    // of one row; requested before the first tile's keys and values.
+    constexpr int kQ = S::kKSteps * NT / kWarps;
+    const int q_row = warp % NT * 8 + g;
+    auto q_step = [&](int x) { return (x * kWarps + warp) / NT; };
+    uint2 qraw[kQ];
+#pragma unroll
+    for (int x = 0; x < kQ; ++x) {
+      // d of the k-step's four elements in lane t: the order of K's 16-byte chunks
+      const int ks = q_step(x);
+      const int d = FP8 ? (ks >> 2) * 64 + t * 16 + (ks & 3) * 4 : (ks >> 1) * 32 + t * 8 + (ks & 1) * 4;
+      const QT* src = qrow + q_row * p.q_sh + d;
+      qraw[x] = make_uint2(0, 0);
+      if (q_row < nq) {
+        if (p.q_vec) {
+          qraw[x] = *reinterpret_cast<const uint2*>(src);
+        } else {
+          QT* e = reinterpret_cast<QT*>(&qraw[x]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) e[j] = src[j];
+        }
+      }
+    }
     if (tile < w_end) {
       find_page(tile);
       load_k(tile);
       load_v(tile);
     }
-
-    // ---- query fragments ----
     __syncthreads();  // the previous item is done with the shared memory
-    // four consecutive elements of a query row
-    auto q4 = [&](int r, int d, float (&v)[4]) {
-      const QT* src = qrow + r * p.q_sh + d;
-      if (p.q_vec) {
-        const uint2 raw = *reinterpret_cast<const uint2*>(src);
-        const QT* e = reinterpret_cast<const QT*>(&raw);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = q_val(e + j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = q_val(src + j);
-      }
-    };
     if constexpr (S::kScaleQ) {
       // power of two that brings each query row's largest value to [1, 2)
-      for (int r = warp; r < S::kHeads; r += kWarps) {
-        float m = 0.0f;
-        if (r < nq) {
-          for (int d = lane * 4; d < D; d += 128) {
-            float v[4];
-            q4(r, d, v);
+      float m = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[j]));
-          }
-        }
+      for (int x = 0; x < kQ; ++x) {
+        const QT* e = reinterpret_cast<const QT*>(&qraw[x]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(q_val(e + j)));
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      if (t == 0) sh_qmax[warp][g] = m;
+      __syncthreads();
+      if (tid < S::kHeads) {
+        float top = 0.0f;
+#pragma unroll
+        for (int w = tid / 8; w < kWarps; w += NT) top = fmaxf(top, sh_qmax[w][tid % 8]);
         int e = 0;
-        if (m > 0.0f && m < INFINITY) e = ilogbf(m);
+        if (top > 0.0f && top < INFINITY) e = ilogbf(top);
         if (e < -100) e = -100;  // rows below 2^-100 keep a factor that fp32 holds
-        if (lane == 0) sh_qexp[r] = ldexpf(1.0f, e);
+        sh_qexp[tid] = ldexpf(1.0f, e);
       }
       __syncthreads();
     }
 #pragma unroll
-    for (int x = 0; x < S::kKSteps * NT * 32 / kThreads; ++x) {
-      const int i = x * kThreads + tid;
-      const int l = i & 31, r = (i >> 5) % NT * 8 + (l >> 2), ks = (i >> 5) / NT;
-      // d of the k-step's four elements in lane t: the order of K's 16-byte chunks
-      const int d = FP8 ? (ks >> 2) * 64 + (l & 3) * 16 + (ks & 3) * 4 : (ks >> 1) * 32 + (l & 3) * 8 + (ks & 1) * 4;
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (r < nq) {
-        q4(r, d, v);
-        if constexpr (S::kScaleQ) {
-          const float f = 1.0f / sh_qexp[r];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] *= f;
-        }
+    for (int x = 0; x < kQ; ++x) {
+      uint2 frag = qraw[x];
+      if constexpr (FP8) {
+        const QT* e = reinterpret_cast<const QT*>(&qraw[x]);
+        const float f = S::kScaleQ ? 1.0f / sh_qexp[q_row] : 1.0f;
+        frag = make_uint2(M::pack(q_val(e) * f, q_val(e + 1) * f), M::pack(q_val(e + 2) * f, q_val(e + 3) * f));
       }
-      sh_q[i] = make_uint2(M::pack(v[0], v[1]), M::pack(v[2], v[3]));
+      sh_q[(q_step(x) * NT + warp % NT) * 32 + lane] = frag;
     }
     __syncthreads();
     float zs[NT][2];  // score factor of this lane's two heads
@@ -526,7 +568,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
     }
 
     // ---- join the warps ----
-    float* mine = sh_part + warp * S::kPart;
+    float* mine = sh_part + warp * S::kPartSh;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -544,8 +586,8 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
           constexpr int per = S::kVV / S::kElem;  // elements of one load
           const int e = 2 * i, c = e / per;
           const int d = c * per * 8 + g * per + e % per;
-          mine[2 * S::kHeads + r * D + d] = o[i][n][j];
-          mine[2 * S::kHeads + r * D + d + 1] = o[i][n][2 + j];
+          mine[2 * S::kHeads + r * S::kPitch + d] = o[i][n][j];
+          mine[2 * S::kHeads + r * S::kPitch + d + 1] = o[i][n][2 + j];
         }
       }
     __syncthreads();
@@ -558,15 +600,15 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
         const int r = i / D, d = i - r * D;
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sh_part[w * S::kPart + r]);
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sh_part[w * S::kPartSh + r]);
         const float ref = mx == -INFINITY ? 0.0f : mx;
         float sum = 0.0f, acc = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float* pt = sh_part + w * S::kPart;
+          const float* pt = sh_part + w * S::kPartSh;
           const float f = exp2_approx(pt[r] - ref);
           sum = fmaf(f, pt[S::kHeads + r], sum);
-          acc = fmaf(f, pt[2 * S::kHeads + r * D + d], acc);
+          acc = fmaf(f, pt[2 * S::kHeads + r * S::kPitch + d], acc);
         }
         if (finish) {
           put(orow + r * p.o_sh + d, sum == 0.0f ? 0.0f : acc / sum * vs);
@@ -579,13 +621,14 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
     };
     // A cut item's parts, joined in CTA order, kJoin at a time: their maxima and sums
     // go to shared memory in one round trip; each thread adds its float4s of the output
-    // with the loads of four parts in flight, against a running maximum per head.
+    // with the loads of several parts in flight, against a running maximum per head.
     auto join_parts = [&](auto&& part_of, int n_parts) {
       constexpr int kJoin = 32;
       float* const sh_m = sh_part;                          // [kJoin][kHeads]
       float* const sh_l = sh_part + kJoin * S::kHeads;      // [kJoin][kHeads]
-      static_assert(2 * kJoin * S::kHeads <= kWarps * S::kPart, "maxima and sums must fit");
+      static_assert(2 * kJoin * S::kHeads <= kWarps * S::kPartSh, "maxima and sums must fit");
       constexpr int kF4 = (S::kHeads * D / 4 + kThreads - 1) / kThreads;  // float4s of a thread
+      constexpr int kAhead = kF4 > 2 ? 4 : 8;                                  // parts whose loads are in flight
       float4 acc[kF4];
       float mx[kF4], sum[kF4];
 #pragma unroll
@@ -610,10 +653,10 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
           acc[x].x *= f0, acc[x].y *= f0, acc[x].z *= f0, acc[x].w *= f0, sum[x] *= f0;
           mx[x] = top;
         }
-        for (int w = 0; w < here; w += 4) {
-          float4 v[4][kF4];
+        for (int w = 0; w < here; w += kAhead) {
+          float4 v[kAhead][kF4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
+          for (int y = 0; y < kAhead; ++y)
 #pragma unroll
             for (int x = 0; x < kF4; ++x) {
               const int e = (x * kThreads + tid) * 4;
@@ -622,7 +665,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
+          for (int y = 0; y < kAhead; ++y) {
             if (w + y >= here) break;
 #pragma unroll
             for (int x = 0; x < kF4; ++x) {
@@ -651,8 +694,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnParams p) {
     } else {
       // CTAs that hold the item's first and last tile
       const long long last_tile = item_first + tiles - 1;
-      const int c_first = static_cast<int>(((item_first + 1) * grid - 1) / T);
-      const int c_last = static_cast<int>(((last_tile + 1) * grid - 1) / T);
+      const int c_first = deal.owner(item_first), c_last = deal.owner(last_tile);
       // slot 0: the item began in an earlier CTA (this CTA's first segment); 1: it begins here
       auto slot = [&](int c) { return p.partials + (static_cast<long long>(c) * 2 + (c == c_first ? 1 : 0)) * S::kPart; };
       join_warps(false, slot(cta));
@@ -705,10 +747,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p) 
   }
   tiles = __shfl_sync(0xffffffffu, tiles, b);
   if (tiles <= kWholeTiles) return;
-  const long long T = units, grid = T < p.grid ? T : p.grid;
+  const Deal deal(units, p.grid);
   const long long first = mine + static_cast<long long>(item) * (tiles + kItemCost) + kItemCost;
-  const int c_first = static_cast<int>(((first + 1) * grid - 1) / T);
-  const int n_parts = static_cast<int>(((first + tiles) * grid - 1) / T) - c_first + 1;
+  const int c_first = deal.owner(first);
+  const int n_parts = deal.owner(first + tiles - 1) - c_first + 1;
   if (n_parts == 1) return;  // stored by its CTA
   auto part_of = [&](int w) { return p.partials + (static_cast<long long>(c_first + w) * 2 + (w == 0 ? 1 : 0)) * S::kPart; };
 
