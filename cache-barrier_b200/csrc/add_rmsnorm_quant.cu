@@ -24,6 +24,7 @@
 
 #include "cb_internal.h"
 #include "cb_ptx.cuh"
+#include "cb_quant8.cuh"
 
 namespace cb {
 namespace {
@@ -92,27 +93,6 @@ __device__ __forceinline__ void store8(T* row, int at, int n, const float (&v)[8
     for (int j = 0; j < 8; ++j)
       if (at + j < n) from_f32(v[j], row[at + j]);
   }
-}
-
-// q = u / step: int8 rounds half away from zero (as the library's other int8
-// quantizers), e4m3 to nearest even; both saturate by construction of the step.
-__device__ __forceinline__ uint64_t quant8(const float (&u)[8], float step, bool int8) {
-  uint64_t out = 0;
-  if (int8) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = __fdiv_rn(u[j], step);
-      const int q = __float2int_rz(__fadd_rn(v, copysignf(0.5f, v)));
-      out |= static_cast<uint64_t>(static_cast<uint8_t>(q)) << (8 * j);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float2 v = make_float2(__fdiv_rn(u[j], step), __fdiv_rn(u[j + 1], step));
-      out |= static_cast<uint64_t>(__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3)) << (8 * j);
-    }
-  }
-  return out;
 }
 
 template <bool VEC>
@@ -209,7 +189,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormParams p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       step[v] = fmaxf(__fdiv_rn(group_max(amax8(u[v])), 448.0f), kNormFloor);
-      store_q8<VEC>(q, (v * blockDim.x + threadIdx.x) * 8, p.H, quant8(u[v], step[v], false));
+      store_q8<VEC>(q, (v * blockDim.x + threadIdx.x) * 8, p.H, quant8<false>(u[v], step[v]));
     }
     row_sum_max(ss, amax, red);
     const float r = row_factor(ss, p.H, p.eps);
@@ -227,9 +207,103 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormParams p) {
     const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      store_q8<VEC>(q, (v * blockDim.x + threadIdx.x) * 8, p.H, quant8(u[v], step, p.int8 != 0));
+      store_q8<VEC>(q, (v * blockDim.x + threadIdx.x) * 8, p.H,
+                    p.int8 ? quant8<true>(u[v], step) : quant8<false>(u[v], step));
     if (threadIdx.x == 0) p.scale[row * p.s_sm] = __fmul_rn(step, row_factor(ss, p.H, p.eps));
   }
+}
+
+// Many rows: CTAs that walk the rows, with the next kAhead rows' loads always in flight.
+// Every thread copies into shared memory just what it will read itself (cp.async), so a
+// row needs no barrier but its reduction's. One CTA per row instead leaves HBM idle
+// while the resident CTAs reduce and store (16384 x 8192 with a residual: 199 us).
+constexpr int kAhead = 2;
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+template <typename T, typename W, bool BLOCK, int NV>
+__global__ void __launch_bounds__(512) norm_rows_kernel(const NormParams p) {
+  extern __shared__ uint4 sh_rows[];  // [kAhead + 1][x, residual][NV][thread]
+  __shared__ float2 red[2][32];
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  const W* w = static_cast<const W*>(p.weight);
+  const int tid = threadIdx.x, n = blockDim.x;
+  auto place = [&](int stage, int which, int v) { return sh_rows + ((stage * 2 + which) * NV + v) * n + tid; };
+  auto request = [&](long long row, int stage) {
+    if (row < p.rows) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int at = (v * n + tid) * 8;
+        if (at >= p.H) continue;
+        cp_async16(place(stage, 0, v), static_cast<const T*>(p.x) + row * p.x_sm + at);
+        if (p.residual) cp_async16(place(stage, 1, v), static_cast<const T*>(p.residual) + row * p.r_sm + at);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) request(blockIdx.x + static_cast<long long>(a) * gridDim.x, a);
+  int stage = 0, parity = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1) {
+    const int last = stage > 0 ? stage - 1 : kAhead;  // the stage before this one: free
+    request(row + static_cast<long long>(kAhead) * gridDim.x, last);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+    T* h = p.h ? static_cast<T*>(p.h) + row * p.h_sm : nullptr;
+    uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.q_sm;
+    float u[NV][8];
+    float ss = 0.0f, amax = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int at = (v * n + tid) * 8;
+      const int left = at < p.H ? 8 : 0;  // rows are whole vectors
+      load8<true>(reinterpret_cast<const T*>(place(stage, 0, v)), 0, left, u[v]);
+      if (p.residual) {
+        float t[8];
+        load8<true>(reinterpret_cast<const T*>(place(stage, 1, v)), 0, left, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[v][j] = __fadd_rn(u[v][j], t[j]);
+        if (h) store8<true>(h, at, p.H, u[v]);
+      }
+      float t[8];
+      load8<true>(w, at, p.H, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        ss = __fmaf_rn(u[v][j], u[v][j], ss);
+        u[v][j] = __fmul_rn(u[v][j], t[j]);
+      }
+    }
+    if constexpr (BLOCK) {
+      float step[NV];
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        step[v] = fmaxf(__fdiv_rn(group_max(amax8(u[v])), 448.0f), kNormFloor);
+        store_q8<true>(q, (v * n + tid) * 8, p.H, quant8<false>(u[v], step[v]));
+      }
+      row_sum_max(ss, amax, red[parity]);
+      const float r = row_factor(ss, p.H, p.eps);
+      if ((tid & 15) == 0) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int at = (v * n + tid) * 8;
+          if (at < p.H) p.scale[row * p.s_sm + at / kGroup] = __fmul_rn(step[v], r);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) amax = fmaxf(amax, amax8(u[v]));
+      row_sum_max(ss, amax, red[parity]);
+      const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        store_q8<true>(q, (v * n + tid) * 8, p.H, p.int8 ? quant8<true>(u[v], step) : quant8<false>(u[v], step));
+      if (tid == 0) p.scale[row * p.s_sm] = __fmul_rn(step, row_factor(ss, p.H, p.eps));
+    }
+    stage = stage == kAhead ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Rows longer than 32768 elements: one CTA per row that reads the row twice (the
@@ -272,7 +346,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_long_kernel(const NormParams
     weighted(at, u, &ss);
     if constexpr (BLOCK) {
       const float step = fmaxf(__fdiv_rn(group_max(amax8(u)), 448.0f), kNormFloor);
-      store_q8<false>(q, at, p.H, quant8(u, step, false));
+      store_q8<false>(q, at, p.H, quant8<false>(u, step));
       if ((threadIdx.x & 15) == 0 && at < p.H) p.scale[row * p.s_sm + at / kGroup] = step;  // times r below
     } else {
       amax = fmaxf(amax, amax8(u));
@@ -291,17 +365,18 @@ __global__ void __launch_bounds__(kMaxThreads) norm_long_kernel(const NormParams
       const long long at = base + threadIdx.x * 8;
       if (at >= p.H) break;
       weighted(static_cast<int>(at), u, nullptr);
-      store_q8<false>(q, static_cast<int>(at), p.H, quant8(u, step, p.int8 != 0));
+      store_q8<false>(q, static_cast<int>(at), p.H, p.int8 ? quant8<true>(u, step) : quant8<false>(u, step));
     }
     if (threadIdx.x == 0) p.scale[row * p.s_sm] = __fmul_rn(step, r);
   }
 }
 
 template <typename K, typename P>
-int launch(K kernel, dim3 grid, dim3 block, cudaStream_t stream, const P& p) {
+int launch(K kernel, dim3 grid, dim3 block, cudaStream_t stream, const P& p, size_t smem = 0) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -311,9 +386,39 @@ int launch(K kernel, dim3 grid, dim3 block, cudaStream_t stream, const P& p) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
+// Rows per CTA from which the walking kernel is used.
+constexpr int kRowsPerCta = 4;
+
+template <typename T, typename W, bool BLOCK, int NV>
+int launch_rows(const NormParams& p, int threads, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(kAhead + 1) * 2 * NV * threads * sizeof(uint4);
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured_dev != dev) {
+    if (cudaFuncSetAttribute(norm_rows_kernel<T, W, BLOCK, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) !=
+        cudaSuccess)
+      return CB_ERR_CUDA;
+    configured_dev = dev;
+  }
+  int per_sm = static_cast<int>((200 * 1024) / smem);
+  if (per_sm > 1024 / threads) per_sm = 1024 / threads;
+  if (per_sm < 1) per_sm = 1;
+  long long grid = static_cast<long long>(sm_count()) * per_sm;
+  if (grid > p.rows) grid = p.rows;
+  return launch(norm_rows_kernel<T, W, BLOCK, NV>, dim3(static_cast<unsigned>(grid)), dim3(threads), stream, p, smem);
+}
+
 template <typename T, typename W, bool BLOCK>
 int launch_norm(const NormParams& p, bool vec, cudaStream_t stream) {
   const int vecs = (p.H + 7) / 8;
+  // 256 or 512 threads and up to four vectors each, three rows of x and residual in shared memory
+  if (vec && vecs > 128 && vecs <= 2048 && p.rows >= static_cast<long long>(sm_count()) * kRowsPerCta * (vecs > 1024 ? 1 : 2)) {
+    const int threads = vecs > 512 ? 512 : 256;  // two vectors a thread where that makes 1024 threads an SM
+    if (vecs <= threads) return launch_rows<T, W, BLOCK, 1>(p, threads, stream);
+    if (vecs <= 2 * threads) return launch_rows<T, W, BLOCK, 2>(p, threads, stream);
+    return launch_rows<T, W, BLOCK, 4>(p, threads, stream);
+  }
   if (vecs > 4 * kMaxThreads)
     return launch(norm_long_kernel<T, W, BLOCK>, dim3(static_cast<unsigned>(p.rows)), dim3(kMaxThreads), stream, p);
   // A warp per row up to 1024 elements; else a CTA per row.
@@ -373,7 +478,7 @@ __global__ void __launch_bounds__(256) quant_block_kernel(const QuantParams p) {
     float v[8];
     load8<VEC>(static_cast<const T*>(p.a) + b * p.a_sb + m * p.a_sm, at, n, v);
     const float s = fmaxf(__fdiv_rn(group_max(amax8(v)), 448.0f), kQuantFloor);
-    store_q8<VEC>(p.q + b * p.q_sb + m * p.q_sm, at, n, quant8(v, s, false));
+    store_q8<VEC>(p.q + b * p.q_sb + m * p.q_sm, at, n, quant8<false>(v, s));
     if (live && lane16 == 0) p.scale[b * p.s_sb + m * p.s_sm + kb] = s;
   }
 }

@@ -5,7 +5,7 @@
 // by the head's scale, saturated, rounded to nearest even.
 //
 // Bound: HBM for many tokens (each element read and written once), launch
-// latency for few. One thread moves eight elements (one 16-byte load).
+// latency for few. One thread moves eight elements at a time (one 16-byte load).
 //
 // A negative slot skips the token (padding of a captured batch). A slot past the
 // cache records CB_DEVERR_BAD_INDEX in *status and is skipped: nothing outside
@@ -14,11 +14,16 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "cb_internal.h"
 #include "cb_ptx.cuh"
+#include "cb_quant8.cuh"
 
 namespace cb {
 namespace {
+
+constexpr int kThreads = 128, kUnroll = 4;
 
 struct AppendParams {
   const void* src[2];  // k, v: [T, heads, D]
@@ -27,9 +32,9 @@ struct AppendParams {
   const void* slots;
   int slots_i64;
   int heads, D, vecs;  // vecs: ceil(D / 8)
-  long long total;     // T * heads * vecs
+  long long T;
   long long capacity;  // pages * page_size
-  int page_size;
+  int page_size, page_shift;  // page_shift: log2 of the page size, or -1
   long long src_st[2], src_sh[2];              // token and head strides
   long long dst_sp[2], dst_ss[2], dst_sh[2];   // page, slot and head strides
   int* status;
@@ -43,41 +48,68 @@ __device__ __forceinline__ void put(__nv_fp8_storage_t* o, float v, float scale)
   *o = __nv_cvt_float_to_fp8(__fdiv_rn(v, scale), __NV_SATFINITE, __NV_E4M3);
 }
 
+// threadIdx.x walks a token's vectors, threadIdx.y and kUnroll its tokens: the slots and
+// rows of kUnroll tokens are all requested before the first is used, and the divisions
+// (vector to head, slot to page) are per thread or token, not per vector.
 template <typename T, typename C, bool VEC>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
   pdl_wait_primary();
   pdl_launch_dependents();
   const int which = blockIdx.y;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < p.total;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long th = i / p.vecs;
-    const int at = static_cast<int>(i - th * p.vecs) * 8;
-    const long long t = th / p.heads;
-    const int h = static_cast<int>(th - t * p.heads);
-    const long long slot = p.slots_i64 ? static_cast<const long long*>(p.slots)[t]
-                                       : static_cast<long long>(static_cast<const int*>(p.slots)[t]);
-    if (slot < 0) continue;
+  const int row = p.heads * p.vecs;  // vectors of a token
+  const long long t0 = (static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y) * kUnroll;
+  long long dst_at[kUnroll];  // element offset of the token's slot; -1: none
+#pragma unroll
+  for (int x = 0; x < kUnroll; ++x) {
+    long long slot = -1;
+    if (t0 + x < p.T)
+      slot = p.slots_i64 ? static_cast<const long long*>(p.slots)[t0 + x] : static_cast<const int*>(p.slots)[t0 + x];
     if (slot >= p.capacity) {
       if (p.status) atomicOr(p.status, CB_DEVERR_BAD_INDEX);
-      continue;
+      slot = -1;
     }
-    const long long page = slot / p.page_size;
-    const T* src = static_cast<const T*>(p.src[which]) + t * p.src_st[which] + h * p.src_sh[which] + at;
-    C* dst = static_cast<C*>(p.dst[which]) + page * p.dst_sp[which] + (slot - page * p.page_size) * p.dst_ss[which] +
-             h * p.dst_sh[which] + at;
-    const float scale = p.scale[which] ? p.scale[which][h] : 1.0f;
+    const long long page = p.page_shift >= 0          ? slot >> p.page_shift
+                           : slot < (1LL << 31)       ? static_cast<int>(slot) / p.page_size
+                                                      : slot / p.page_size;
+    dst_at[x] = slot < 0 ? -1 : page * p.dst_sp[which] + (slot - page * p.page_size) * p.dst_ss[which];
+  }
+  for (int i = threadIdx.x; i < row; i += blockDim.x) {
+    const int h = i / p.vecs, at = (i - h * p.vecs) * 8;
+    const T* src = static_cast<const T*>(p.src[which]) + t0 * p.src_st[which] + h * p.src_sh[which] + at;
+    C* dst = static_cast<C*>(p.dst[which]) + h * p.dst_sh[which] + at;
+    const float scale = p.scale[which] ? __ldg(p.scale[which] + h) : 1.0f;
     if constexpr (VEC) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(src);
-      const T* e = reinterpret_cast<const T*>(&raw);
-      struct alignas(8 * sizeof(C)) Out {
-        C v[8];
-      } out;
+      uint4 raw[kUnroll];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) put(&out.v[j], to_f32(e[j]), scale);
-      *reinterpret_cast<Out*>(dst) = out;
+      for (int x = 0; x < kUnroll; ++x)
+        raw[x] = dst_at[x] >= 0 ? *reinterpret_cast<const uint4*>(src + x * p.src_st[which]) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < kUnroll; ++x) {
+        if (dst_at[x] < 0) continue;
+        const T* e = reinterpret_cast<const T*>(&raw[x]);
+        struct alignas(8 * sizeof(C)) Out {
+          C v[8];
+        } out;
+        if constexpr (std::is_same<T, C>::value) {
+          out = *reinterpret_cast<const Out*>(&raw[x]);
+        } else if constexpr (sizeof(C) == 1) {
+          float u[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u[j] = to_f32(e[j]);
+          const uint64_t q = quant8<false>(u, scale);
+          out = *reinterpret_cast<const Out*>(&q);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) put(&out.v[j], to_f32(e[j]), scale);
+        }
+        *reinterpret_cast<Out*>(dst + dst_at[x]) = out;
+      }
     } else {
       const int n = p.D - at < 8 ? p.D - at : 8;
-      for (int j = 0; j < n; ++j) put(dst + j, to_f32(src[j]), scale);
+      for (int x = 0; x < kUnroll; ++x) {
+        if (dst_at[x] < 0) continue;
+        for (int j = 0; j < n; ++j) put(dst + dst_at[x] + j, to_f32(src[x * p.src_st[which] + j]), scale);
+      }
     }
   }
 }
@@ -85,9 +117,11 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 template <typename T, typename C>
 int launch_append(const AppendParams& p, bool vec, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  const long long blocks = (p.total + 255) / 256;
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20)), 2);
-  cfg.blockDim = dim3(256);
+  int tx = 8;  // threads along a token's vectors: a power of two
+  while (tx < kThreads && tx < p.heads * p.vecs) tx *= 2;
+  const int tokens = kThreads / tx * kUnroll;
+  cfg.gridDim = dim3(static_cast<unsigned>((p.T + tokens - 1) / tokens), 2);
+  cfg.blockDim = dim3(tx, kThreads / tx);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -132,9 +166,12 @@ extern "C" CB_API int cb_paged_kv_append(const void* k, const void* v, int dtype
   p.heads = static_cast<int>(heads);
   p.D = static_cast<int>(D);
   p.vecs = static_cast<int>((D + 7) / 8);
-  p.total = T * heads * p.vecs;
+  p.T = T;
   p.capacity = num_pages * page_size;
   p.page_size = static_cast<int>(page_size);
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (page_size == (1LL << s)) p.page_shift = s;
   const int64_t ce = cache_dtype == CB_DTYPE_E4M3 ? 1 : 2;
   bool vec = D % 8 == 0;
   for (int i = 0; i < 2; ++i) {

@@ -83,6 +83,18 @@ def test_norm_matches_formula(cuda_device, rows, H, dtype, mode):
     _check(ops.add_rmsnorm_quant(xd, wd, 1e-5, mode=mode), _reference(x, w, 1e-5, None, mode))
 
 
+@pytest.mark.parametrize("mode", ["int8", "fp8", "fp8_block"])
+@pytest.mark.parametrize("dtype,w_dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("rows,H", [(1300, 1032), (1201, 4000), (2500, 8192), (1184, 16384), (5000, 2048), (3000, 512)])
+def test_norm_many_rows(cuda_device, rows, H, dtype, w_dtype, mode):
+    from cb200 import ops
+    x, w, res = _inputs(rows, H, dtype, w_dtype, rows + H)
+    x[rows // 2] *= 100.0  # a row of another scale in the middle of a CTA's rows
+    xd, wd, rd = _dev(cuda_device, x, w, res)
+    _check(ops.add_rmsnorm_quant(xd, wd, 1e-6, residual=rd, mode=mode, h=rd), _reference(x, w, 1e-6, res, mode))
+    _check(ops.add_rmsnorm_quant(xd, wd, 1e-6, mode=mode), _reference(x, w, 1e-6, None, mode))
+
+
 @pytest.mark.parametrize("w_dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("mode", ["int8", "fp8_block"])
 def test_norm_weight_types(cuda_device, w_dtype, mode):
