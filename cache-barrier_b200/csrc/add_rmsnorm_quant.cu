@@ -213,24 +213,31 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormParams p) {
   }
 }
 
-// Many rows: CTAs that walk the rows, with the next kAhead rows' loads always in flight.
+// Many rows: CTAs that walk the rows, with the next AHEAD rows' loads always in flight.
 // Every thread copies into shared memory just what it will read itself (cp.async), so a
 // row needs no barrier but its reduction's. One CTA per row instead leaves HBM idle
 // while the resident CTAs reduce and store (16384 x 8192 with a residual: 199 us).
-constexpr int kAhead = 2;
-
+// The weight stays in registers.
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
-template <typename T, typename W, bool BLOCK, int NV>
-__global__ void __launch_bounds__(512) norm_rows_kernel(const NormParams p) {
-  extern __shared__ uint4 sh_rows[];  // [kAhead + 1][x, residual][NV][thread]
+template <typename T, typename W, bool BLOCK, int NV, int AHEAD>
+__global__ void __launch_bounds__(512, NV == 4 ? 1 : 2) norm_rows_kernel(const NormParams p) {
+  extern __shared__ uint4 sh_rows[];  // [AHEAD + 1][x, residual][NV][thread]
   __shared__ float2 red[2][32];
   pdl_wait_primary();
   pdl_launch_dependents();
-  const W* w = static_cast<const W*>(p.weight);
   const int tid = threadIdx.x, n = blockDim.x;
+  constexpr int kWv = sizeof(W) * 8 / 16;  // 16-byte pieces of eight weights
+  uint4 wraw[NV][kWv];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int i = 0; i < kWv; ++i) {
+      const int at = (v * n + tid) * 8;
+      wraw[v][i] = at < p.H ? reinterpret_cast<const uint4*>(static_cast<const W*>(p.weight) + at)[i] : make_uint4(0, 0, 0, 0);
+    }
   auto place = [&](int stage, int which, int v) { return sh_rows + ((stage * 2 + which) * NV + v) * n + tid; };
   auto request = [&](long long row, int stage) {
     if (row < p.rows) {
@@ -245,12 +252,12 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(const NormParams p) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int a = 0; a < kAhead; ++a) request(blockIdx.x + static_cast<long long>(a) * gridDim.x, a);
+  for (int a = 0; a < AHEAD; ++a) request(blockIdx.x + static_cast<long long>(a) * gridDim.x, a);
   int stage = 0, parity = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1) {
-    const int last = stage > 0 ? stage - 1 : kAhead;  // the stage before this one: free
-    request(row + static_cast<long long>(kAhead) * gridDim.x, last);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+    const int last = stage > 0 ? stage - 1 : AHEAD;  // the stage before this one: free
+    request(row + static_cast<long long>(AHEAD) * gridDim.x, last);
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
     T* h = p.h ? static_cast<T*>(p.h) + row * p.h_sm : nullptr;
     uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.q_sm;
     float u[NV][8];
@@ -268,7 +275,9 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(const NormParams p) {
         if (h) store8<true>(h, at, p.H, u[v]);
       }
       float t[8];
-      load8<true>(w, at, p.H, t);
+      const W* w = reinterpret_cast<const W*>(wraw[v]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = to_f32(w[j]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         ss = __fmaf_rn(u[v][j], u[v][j], ss);
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(512) norm_rows_kernel(const NormParams p) {
         store_q8<true>(q, (v * n + tid) * 8, p.H, p.int8 ? quant8<true>(u[v], step) : quant8<false>(u[v], step));
       if (tid == 0) p.scale[row * p.s_sm] = __fmul_rn(step, row_factor(ss, p.H, p.eps));
     }
-    stage = stage == kAhead ? 0 : stage + 1;
+    stage = stage == AHEAD ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -389,38 +398,41 @@ int launch(K kernel, dim3 grid, dim3 block, cudaStream_t stream, const P& p, siz
 // Rows per CTA from which the walking kernel is used.
 constexpr int kRowsPerCta = 4;
 
-template <typename T, typename W, bool BLOCK, int NV>
-int launch_rows(const NormParams& p, int threads, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(kAhead + 1) * 2 * NV * threads * sizeof(uint4);
+template <typename T, typename W, bool BLOCK, int NV, int AHEAD>
+int launch_rows(const NormParams& p, cudaStream_t stream) {
+  const int threads = ((p.H / 8 + NV - 1) / NV + 31) / 32 * 32;
+  const size_t smem = static_cast<size_t>(AHEAD + 1) * 2 * NV * threads * sizeof(uint4);
   static thread_local int configured_dev = -1;
   int dev = 0;
   cudaGetDevice(&dev);
   if (configured_dev != dev) {
-    if (cudaFuncSetAttribute(norm_rows_kernel<T, W, BLOCK, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) !=
-        cudaSuccess)
+    if (cudaFuncSetAttribute(norm_rows_kernel<T, W, BLOCK, NV, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             200 * 1024) != cudaSuccess)
       return CB_ERR_CUDA;
     configured_dev = dev;
   }
-  int per_sm = static_cast<int>((200 * 1024) / smem);
-  if (per_sm > 1024 / threads) per_sm = 1024 / threads;
-  if (per_sm < 1) per_sm = 1;
+  int per_sm = 1;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, norm_rows_kernel<T, W, BLOCK, NV, AHEAD>, threads, smem) !=
+          cudaSuccess || per_sm < 1)
+    return CB_ERR_CUDA;
   long long grid = static_cast<long long>(sm_count()) * per_sm;
   if (grid > p.rows) grid = p.rows;
-  return launch(norm_rows_kernel<T, W, BLOCK, NV>, dim3(static_cast<unsigned>(grid)), dim3(threads), stream, p, smem);
+  return launch(norm_rows_kernel<T, W, BLOCK, NV, AHEAD>, dim3(static_cast<unsigned>(grid)), dim3(threads), stream, p, smem);
 }
 
 template <typename T, typename W, bool BLOCK>
 int launch_norm(const NormParams& p, bool vec, cudaStream_t stream) {
   const int vecs = (p.H + 7) / 8;
-  // 256 or 512 threads and up to four vectors each, three rows of x and residual in shared memory
-  if (vec && vecs > 128 && vecs <= 2048 && p.rows >= static_cast<long long>(sm_count()) * kRowsPerCta * (vecs > 1024 ? 1 : 2)) {
-    const int threads = vecs > 512 ? 512 : 256;  // two vectors a thread where that makes 1024 threads an SM
-    if (vecs <= threads) return launch_rows<T, W, BLOCK, 1>(p, threads, stream);
-    if (vecs <= 2 * threads) return launch_rows<T, W, BLOCK, 2>(p, threads, stream);
-    return launch_rows<T, W, BLOCK, 4>(p, threads, stream);
-  }
   if (vecs > 4 * kMaxThreads)
     return launch(norm_long_kernel<T, W, BLOCK>, dim3(static_cast<unsigned>(p.rows)), dim3(kMaxThreads), stream, p);
+  // Up to 512 threads of one, two or four vectors. Short rows keep two more in flight,
+  // longer ones one more (8192 elements: 144 us with one, 173 us with three: the more
+  // CTAs then fit an SM).
+  if (vec && vecs > 128 && vecs <= 2048 && p.rows >= static_cast<long long>(sm_count()) * kRowsPerCta * (vecs > 1024 ? 1 : 2)) {
+    if (vecs <= 256) return launch_rows<T, W, BLOCK, 1, 2>(p, stream);
+    if (vecs <= 1024) return launch_rows<T, W, BLOCK, 2, 1>(p, stream);
+    return launch_rows<T, W, BLOCK, 4, 1>(p, stream);
+  }
   // A warp per row up to 1024 elements; else a CTA per row.
   const bool warp_rows = vecs <= 32 * 4;
   int nv = 4;
