@@ -19,6 +19,32 @@ struct BlockGemmArgs {
   void* workspace;
 };
 
+// What joining a tile's parts costs, in k-blocks: `join`, and `each` for every `per`
+// parts after the first.
+struct JoinCost {
+  int join, per, each;
+  long long of(long long parts) const { return parts < 2 ? 0 : join + each * ((parts - 1 + per - 1) / per); }
+};
+
+// CTAs that share the k-blocks of all tiles, end to end, in equal ranges.
+struct SplitPlan {
+  int grid;
+  long long cost;  // k-blocks of the busiest CTA, with its join
+};
+
+// Either x CTAs for every tile, so that ranges end where tiles do, or all `sms`, whose
+// ranges cut the tiles anywhere (a part more per tile).
+inline SplitPlan plan_split(long long tiles, long long KB, int sms, const JoinCost& c) {
+  const long long total = tiles * KB;
+  SplitPlan best = {static_cast<int>(total < sms ? total : sms),
+                    (total + sms - 1) / sms + c.of((sms + tiles - 1) / tiles + 1)};
+  for (long long x = 1; x <= KB && tiles * x <= sms; ++x) {
+    const long long cost = (KB + x - 1) / x + c.of(x);
+    if (cost <= best.cost) best = {static_cast<int>(tiles * x), cost};
+  }
+  return best;
+}
+
 // 128-element blocks of K that the busiest CTA (pair) works through.
 long long block_gemm_pair_blocks(const BlockGemmArgs& L);
 long long block_gemm_tc_blocks(const BlockGemmArgs& L);

@@ -9,7 +9,8 @@
 // to fp32 totals in registers.
 //
 // The (128 channels, k-block) units of all tiles are laid end to end and dealt to the
-// CTAs (one per SM) in equal contiguous ranges; cut tiles are reduced as
+// CTAs (at most one per SM, as many as pay for the join: plan_split) in equal contiguous
+// ranges; cut tiles are reduced as
 // cb_gemm_common.cuh describes (parts published early, the first contributor adds
 // them in CTA order after a short bounded poll, else the last to arrive does), so no
 // CTA waits for one that may not run, and the bits do not depend on who adds.
@@ -295,16 +296,16 @@ __global__ void __launch_bounds__(kThreads<TN>, kPerSm<TN>)
     auto slot = [&](int c, int c_first) {
       return p.partials + (static_cast<long long>(c) * 2 + (c == c_first ? 1 : 0)) * (TN * kBlk) + group * TC * kBlk + row;
     };
-    // sum = the parts of c_first .. c_last in order; `me`'s is in sum (-1: all are published)
-    auto add_parts = [&](int c_first, int c_last, int me) {
+    // sum = the parts of c_first .. c_last in order; the first is in sum if `held`
+    auto add_parts = [&](int c_first, int c_last, bool held) {
       constexpr int kStep = 8, kAhead = 4;  // tokens and parts whose loads are in flight together
 #pragma unroll
       for (int c = 0; c < TC; c += kStep) {
         if (c >= M) break;
         float v[kStep];
 #pragma unroll
-        for (int x = 0; x < kStep; ++x) v[x] = 0.0f;
-        for (int q0 = c_first; q0 <= c_last; q0 += kAhead) {
+        for (int x = 0; x < kStep; ++x) v[x] = 0.0f + (held ? sum[c + x] : 0.0f);
+        for (int q0 = held ? c_first + 1 : c_first; q0 <= c_last; q0 += kAhead) {
           float part[kAhead][kStep];
 #pragma unroll
           for (int q = 0; q < kAhead; ++q) {
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kThreads<TN>, kPerSm<TN>)
           for (int q = 0; q < kAhead; ++q)
             if (q0 + q <= c_last) {
 #pragma unroll
-              for (int x = 0; x < kStep; ++x) v[x] += q0 + q == me ? sum[c + x] : part[q][x];
+              for (int x = 0; x < kStep; ++x) v[x] += part[q][x];
             }
         }
 #pragma unroll
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(kThreads<TN>, kPerSm<TN>)
             if (last) __threadfence();
           }
           if (last) {
-            if (live) add_parts(c_first, c_last, me);
+            if (live) add_parts(c_first, c_last, true);
             if (threadIdx.x == leader) counters[c_first] = 0;  // the next launch starts from zero
           }
           emit = emit && last;
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(kThreads<TN>, kPerSm<TN>)
       named_bar_sync(ebar, 128);
       if (sh_last[group]) {
         __threadfence();
-        add_parts(pend_first, pend_last, -1);
+        add_parts(pend_first, pend_last, false);
         if (threadIdx.x == leader) counters[pend_first] = 0;
         store_out(static_cast<int>(pend_tile / p.n_tiles), static_cast<int>(pend_tile % p.n_tiles));
       }
@@ -491,8 +492,14 @@ int launch_block_gemm_decode(const BlockGemmArgs& L, cudaStream_t stream) {
   p.KB = static_cast<int>((L.K + kBlk - 1) / kBlk);
   p.n_tiles = static_cast<int>((L.N + kBlk - 1) / kBlk);
   p.sk.total = L.batch * static_cast<long long>(p.n_tiles) * p.KB;
-  int grid = sms < kMaxGrid / 2 ? sms : kMaxGrid / 2;  // two counters a CTA
-  if (p.sk.total < grid) grid = static_cast<int>(p.sk.total);
+  // A join takes as long as 8 blocks (0.28 us each) and, for every four parts, 1 to 4
+  // more. With K = 4096, N = 4096 and one token: 13.4 us whole, 8.7 in four parts a
+  // tile, 9.0 on all SMs; 64 tokens 16.8, 12.7, 14.3. With K = 1024, N = 9000: 6.0
+  // whole and 7.8 on all SMs. With K = 17408, N = 256 and 64 tokens 16.7 in nine parts
+  // a tile, 46.3 on all SMs.
+  const SplitPlan split = plan_split(L.batch * p.n_tiles, p.KB, sms < kMaxGrid / 2 ? sms : kMaxGrid / 2,  // two counters a CTA
+                                     {8, 4, L.M <= 16 ? 1 : L.M <= 32 ? 2 : 4});
+  const int grid = split.grid;
   p.sk.grid = grid;
   p.sk.kb_per_tile = p.KB;
   p.a_scale = L.a_scale, p.as_sb = L.as_sb, p.as_sm = L.as_sm;

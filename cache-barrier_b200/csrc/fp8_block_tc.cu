@@ -15,8 +15,8 @@
 // accumulator, two produce and two wait for accumulators, all on alternate blocks.
 //
 // CTAs take whole tiles, or, where that leaves SMs idle, the k-blocks of all tiles end
-// to end in one contiguous range per CTA (cb_gemm_common.cuh): parts of a cut tile are
-// published as they end, and the tile's first contributor adds them in CTA order after
+// to end in one contiguous range per CTA (cb_gemm_common.cuh), as many CTAs as pay for
+// the join (plan_split): parts of a cut tile are published as they end, and the tile's first contributor adds them in CTA order after
 // a short bounded poll, else the last to arrive does. No CTA waits for one that may
 // not run, and the bits do not depend on who adds.
 //
@@ -38,6 +38,9 @@ constexpr int kBM = 128, kBN = 128, kBK = 128;
 constexpr int kStages = 6;
 constexpr int kAcc = 4;  // accumulators in tensor memory, one per MMA issuer
 constexpr int kThreads = 512;
+// Registers: 512 x 128 at launch = 256 x 80 + 256 x 176. The epilogue holds 64 totals and
+// an accumulator's 64 columns, or two parts' quarters in flight.
+constexpr int kRegsFirst = 80, kRegsEpi = 176;
 constexpr int kTC = 64;  // channels per epilogue warpgroup
 constexpr int kHandBar = 2, kHandThreads = 32 + 256;
 constexpr int kGroupM = 16;  // m-tiles that neighbouring CTAs share weight tiles over
@@ -47,7 +50,6 @@ struct TcParams {
   int M, N, KB;
   int m_tiles, n_tiles;
   long long tiles;
-  int whole;  // CTAs take whole tiles cta, cta + grid, ...; else stream-K ranges
   StreamK sk;
   const float* a_scale;
   long long as_sb, as_sm;
@@ -91,11 +93,12 @@ __device__ __forceinline__ void tile_of(const TcParams& p, long long tile, int& 
 }
 
 // A unit (tile, k-block) of this CTA, advanced one or several at a time.
+template <bool SPLIT>
 struct Unit {
   long long tile;
   int kb, b, mt, nt;
   __device__ __forceinline__ Unit(const TcParams& p, int skip) {
-    if (p.whole) {
+    if (!SPLIT) {
       tile = blockIdx.x;
       kb = 0;
     } else {
@@ -111,12 +114,14 @@ struct Unit {
     if (kb < p.KB) return;
     do {
       kb -= p.KB;
-      tile += p.whole ? static_cast<int>(gridDim.x) : 1;
+      tile += SPLIT ? 1 : static_cast<int>(gridDim.x);
     } while (kb >= p.KB);
     if (tile < p.tiles) tile_of(p, tile, b, mt, nt);  // (past the CTA's last unit it is not used)
   }
 };
 
+// SPLIT: a contiguous range of k-blocks per CTA; else whole tiles cta, cta + grid, ...
+template <bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                          const TcParams p) {
@@ -129,8 +134,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = p.whole ? static_cast<int>(((p.tiles - 1 - blockIdx.x) / gridDim.x + 1) * p.KB)
-                            : static_cast<int>(p.sk.start(blockIdx.x + 1) - p.sk.start(blockIdx.x));
+  const int units = SPLIT ? static_cast<int>(p.sk.start(blockIdx.x + 1) - p.sk.start(blockIdx.x))
+                          : static_cast<int>(((p.tiles - 1 - blockIdx.x) / gridDim.x + 1) * p.KB);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -158,86 +163,90 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
 
-  if (warp == 0 || warp == 12) {
-    // ---------------- TMA producers: the first ring pass by the lanes of warp 0, then units j, j + 2, ... ----------------
-    const int j = warp == 0 ? 0 : 1;
-    const uint64_t pol = policy_evict_normal();
-    auto fill = [&](const Unit& u, int stage) {
-      mbar_arrive_expect_tx(&full_bar[stage], kStageBytes);
-      uint8_t* dst = smem + stage * kStageBytes;
-      tma_load_3d(dst, &tmap_a, &full_bar[stage], u.kb * kBK, u.mt * kBM, u.b, pol);
-      tma_load_3d(dst + kTileBytes, &tmap_w, &full_bar[stage], u.kb * kBK, u.nt * kBN, u.b, pol);
-    };
-    const Unit first(p, j == 0 && lane < kStages && lane < units ? lane : 0);
-    Unit u(p, kStages + j < units ? kStages + j : 0);
-    pdl_wait_primary();
-    if (threadIdx.x == 0) pdl_launch_dependents();
-    __syncwarp();
-    if (j == 0 && lane < kStages && lane < units) fill(first, lane);
-    __syncwarp();
-    if (lane == 0) {
-      int i = kStages + j;
-      for (; i < units; i += 2) {
-        const int stage = i % kStages;
-        if (!mbar_wait_quick(&empty_bar[stage], static_cast<uint32_t>((i / kStages - 1) & 1), abort_ptr, p.status)) break;
-        fill(u, stage);
-        u.advance(p, 2);
+  if (warp < 4 || warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFirst));
+    if (warp == 0 || warp == 12) {
+      // ---------------- TMA producers: the first ring pass by the lanes of warp 0, then units j, j + 2, ... ----------------
+      const int j = warp == 0 ? 0 : 1;
+      const uint64_t pol = policy_evict_normal();
+      auto fill = [&](const Unit<SPLIT>& u, int stage) {
+        mbar_arrive_expect_tx(&full_bar[stage], kStageBytes);
+        uint8_t* dst = smem + stage * kStageBytes;
+        tma_load_3d(dst, &tmap_a, &full_bar[stage], u.kb * kBK, u.mt * kBM, u.b, pol);
+        tma_load_3d(dst + kTileBytes, &tmap_w, &full_bar[stage], u.kb * kBK, u.nt * kBN, u.b, pol);
+      };
+      const Unit<SPLIT> first(p, j == 0 && lane < kStages && lane < units ? lane : 0);
+      Unit<SPLIT> u(p, kStages + j < units ? kStages + j : 0);
+      pdl_wait_primary();
+      if (threadIdx.x == 0) pdl_launch_dependents();
+      __syncwarp();
+      if (j == 0 && lane < kStages && lane < units) fill(first, lane);
+      __syncwarp();
+      if (lane == 0) {
+        int i = kStages + j;
+        for (; i < units; i += 2) {
+          const int stage = i % kStages;
+          if (!mbar_wait_quick(&empty_bar[stage], static_cast<uint32_t>((i / kStages - 1) & 1), abort_ptr, p.status)) break;
+          fill(u, stage);
+          u.advance(p, 2);
+        }
+        sh_issued[j] = i < units ? i : units;  // this warp's units below that are issued
       }
-      sh_issued[j] = i < units ? i : units;  // this warp's units below that are issued
-    }
-    __syncwarp();
-  } else if (warp < 4 || warp == 13) {
-    // ---------------- MMA issuers: accumulator j, units j, j + 4, ... ----------------
-    const int j = warp == 13 ? 3 : warp - 1;
-    pdl_wait_primary();
-    int i = j;
-    if (lane == 0) {
-      const uint32_t idesc = idesc_e4m3_f32(kBM, kBN);
-      for (; i < units; i += kAcc) {
-        const int stage = i % kStages;
-        if (!mbar_wait_quick(&tempty_bar[j], static_cast<uint32_t>((i / kAcc) & 1) ^ 1u, abort_ptr, p.status) ||
-            !mbar_wait_quick(&full_bar[stage], static_cast<uint32_t>((i / kStages) & 1), abort_ptr, p.status))
-          break;
-        tc_fence_after();
-        const uint32_t sa = smem_u32(smem + stage * kStageBytes), sw = sa + kTileBytes;
+      __syncwarp();
+    } else if (warp < 4 || warp == 13) {
+      // ---------------- MMA issuers: accumulator j, units j, j + 4, ... ----------------
+      const int j = warp == 13 ? 3 : warp - 1;
+      pdl_wait_primary();
+      int i = j;
+      if (lane == 0) {
+        const uint32_t idesc = idesc_e4m3_f32(kBM, kBN);
+        for (; i < units; i += kAcc) {
+          const int stage = i % kStages;
+          if (!mbar_wait_quick(&tempty_bar[j], static_cast<uint32_t>((i / kAcc) & 1) ^ 1u, abort_ptr, p.status) ||
+              !mbar_wait_quick(&full_bar[stage], static_cast<uint32_t>((i / kStages) & 1), abort_ptr, p.status))
+            break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * kStageBytes), sw = sa + kTileBytes;
 #pragma unroll
-        for (int kk = 0; kk < kBK / 32; ++kk)
-          mma_f8_ss(tmem + j * kBN, smem_desc_sw128(sa + kk * 32), smem_desc_sw128(sw + kk * 32), idesc, kk != 0);
-        mma_commit(&tfull_bar[j]);
-        mma_commit(&empty_bar[stage]);
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            mma_f8_ss(tmem + j * kBN, smem_desc_sw128(sa + kk * 32), smem_desc_sw128(sw + kk * 32), idesc, kk != 0);
+          mma_commit(&tfull_bar[j]);
+          mma_commit(&empty_bar[stage]);
+        }
+        sh_consumed[j] = i;  // first unit of this warp's that was not issued
+        mma_commit(&drain_bar[j]);
       }
-      sh_consumed[j] = i;  // first unit of this warp's that was not issued
-      mma_commit(&drain_bar[j]);
-    }
-    // Every commit's arrival must land before the CTA exits: the MMAs' end, the last
-    // use of each stage (waited for by the warp that issued it) and the last hand-off.
-    i = __shfl_sync(0xffffffffu, i, 0);
-    if (lane == 31) mbar_wait_quick(&drain_bar[j], 0, nullptr, p.status);
-    const int js = i - kAcc - kAcc * lane;
-    if (lane < 2 && js >= 0 && js + kStages >= units)
-      mbar_wait_quick(&empty_bar[js % kStages], static_cast<uint32_t>((js / kStages) & 1), nullptr, p.status);
-    if (lane == 16 && i >= kAcc) mbar_wait_quick(&tfull_bar[j], static_cast<uint32_t>(((i - kAcc) / kAcc) & 1), nullptr, p.status);
-    __syncwarp();
-  } else if (warp >= 14) {
-    // ---------------- accumulator waiters: hand over the units j, j + 2, ... ----------------
-    const int j = warp - 14;
-    pdl_wait_primary();
-    for (int i = j; i < units; i += 2) {
-      bool ok = true;
-      if (lane == 0) ok = mbar_wait_quick(&tfull_bar[i % kAcc], static_cast<uint32_t>((i / kAcc) & 1), abort_ptr, p.status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (named_bar_or(kHandBar + j, kHandThreads, !ok)) break;
+      // Every commit's arrival must land before the CTA exits: the MMAs' end, the last
+      // use of each stage (waited for by the warp that issued it) and the last hand-off.
+      i = __shfl_sync(0xffffffffu, i, 0);
+      if (lane == 31) mbar_wait_quick(&drain_bar[j], 0, nullptr, p.status);
+      const int js = i - kAcc - kAcc * lane;
+      if (lane < 2 && js >= 0 && js + kStages >= units)
+        mbar_wait_quick(&empty_bar[js % kStages], static_cast<uint32_t>((js / kStages) & 1), nullptr, p.status);
+      if (lane == 16 && i >= kAcc) mbar_wait_quick(&tfull_bar[j], static_cast<uint32_t>(((i - kAcc) / kAcc) & 1), nullptr, p.status);
+      __syncwarp();
+    } else if (warp >= 14) {
+      // ---------------- accumulator waiters: hand over the units j, j + 2, ... ----------------
+      const int j = warp - 14;
+      pdl_wait_primary();
+      for (int i = j; i < units; i += 2) {
+        bool ok = true;
+        if (lane == 0) ok = mbar_wait_quick(&tfull_bar[i % kAcc], static_cast<uint32_t>((i / kAcc) & 1), abort_ptr, p.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (named_bar_or(kHandBar + j, kHandThreads, !ok)) break;
+      }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     // ---------------- epilogue: one token per thread, 64 channels per warpgroup ----------------
     const int group = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int leader = 128 + group * 128, ebar = 4 + group;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + group * kTC;
     int* const counters = p.counters + group * (kMaxGrid / 2);  // one counter per group: groups finish on their own
-    Unit u(p, 0);
+    Unit<SPLIT> u(p, 0);
     // contributors of the tiles that this CTA's range begins and ends in
     long long cc_a = 0, cc_z = 0;
-    if (!p.whole) {
+    if (SPLIT) {
       cc_a = cut_contributors(p.sk.total, p.sk.grid, p.KB, u.tile);
       cc_z = cut_contributors(p.sk.total, p.sk.grid, p.KB, (p.sk.start(blockIdx.x + 1) - 1) / p.KB);
     }
@@ -248,28 +257,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto slot = [&](int c, int c_first) {
       return p.partials + (static_cast<long long>(c) * 2 + (c == c_first ? 1 : 0)) * (kBN * kBM) + group * kTC * kBM + row;
     };
-    // sum = the parts of c_first .. c_last in order; `me`'s is in sum (-1: all are published)
-    auto add_parts = [&](int c_first, int c_last, int me, bool row_live) {
+    // sum = the parts of c_first .. c_last in order; the first is in sum if `held`. A
+    // quarter of the channels at a time, each part's requested two ahead of its addition.
+    auto add_parts = [&](int c_first, int c_last, bool held, bool row_live) {
+      constexpr int kAt = 16, kParts = 2;
+      const int from = held ? c_first + 1 : c_first;
 #pragma unroll
-      for (int c = 0; c < kTC; c += 8) {
-        float v[8] = {};
-        for (int q0 = c_first; q0 <= c_last; q0 += 4) {
-          float part[4][8];
+      for (int x0 = 0; x0 < kTC; x0 += kAt) {
+        float v[kAt], buf[kParts][kAt];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float* src = slot(q0 + q <= c_last ? q0 + q : c_last, c_first) + c * kBM;
+        for (int x = 0; x < kAt; ++x) v[x] = 0.0f + (held ? sum[x0 + x] : 0.0f);
+        auto load = [&](int c, float (&to)[kAt]) {
+          const float* src = slot(c, c_first) + x0 * kBM;
+          const bool on = row_live && c <= c_last;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) part[q][x] = row_live ? __ldcg(src + x * kBM) : 0.0f;
+          for (int x = 0; x < kAt; ++x) to[x] = on ? __ldcg(src + x * kBM) : 0.0f;
+        };
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) load(from + q, buf[q]);
+        for (int c = from; c <= c_last; c += kParts) {
+#pragma unroll
+          for (int q = 0; q < kParts; ++q) {
+#pragma unroll
+            for (int x = 0; x < kAt; ++x) v[x] += buf[q][x];
+            load(c + q + kParts, buf[q]);
           }
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q0 + q <= c_last) {
-#pragma unroll
-              for (int x = 0; x < 8; ++x) v[x] += q0 + q == me ? sum[c + x] : part[q][x];
-            }
         }
 #pragma unroll
-        for (int x = 0; x < 8; ++x) sum[c + x] = v[x];
+        for (int x = 0; x < kAt; ++x) sum[x0 + x] = v[x];
       }
     };
     auto store_out = [&](int b, int mt, int nt) {
@@ -347,21 +362,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!live) break;
         if (some) {
           tc_fence_after();
+          uint32_t r[2][32];
+          tmem_ld32(lane_addr + acc * kBN, r[0]);
+          tmem_ld32(lane_addr + acc * kBN + 32, r[1]);
+          tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < kTC; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(lane_addr + acc * kBN + c, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) sum[c + x] = fmaf(__uint_as_float(r[x]), f, sum[c + x]);
-          }
+          for (int x = 0; x < kTC; ++x) sum[x] = fmaf(__uint_as_float(r[x / 32][x % 32]), f, sum[x]);
           tc_fence_before();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&tempty_bar[acc]);
       }
       bool emit = live;
-      if (here != p.KB) {
+      if (SPLIT && here != p.KB) {
         const long long cc = i == 0 ? cc_a : cc_z;
         const int c_first = static_cast<int>(cc & 0xffffffffLL), c_last = static_cast<int>(cc >> 32);
         const int n_parts = c_last - c_first + 1, me = static_cast<int>(blockIdx.x);
@@ -389,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (last) __threadfence();
           }
           if (last) {
-            if (live) add_parts(c_first, c_last, me, row_live);
+            if (live) add_parts(c_first, c_last, true, row_live);
             if (threadIdx.x == leader) counters[c_first] = 0;  // the next launch starts from zero
           }
           emit = emit && last;
@@ -402,14 +415,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // The part published without looking: if it was the tile's last to arrive (the
     // first contributor gave up its poll), the tile is reduced here.
-    if (pend_tile >= 0) {
+    if (SPLIT && pend_tile >= 0) {
       if (threadIdx.x == leader) sh_last[group] = !*abort_ptr && pend_old == pend_last - pend_first;
       named_bar_sync(ebar, 128);
       if (sh_last[group]) {
         __threadfence();
         int b, mt, nt;
         tile_of(p, pend_tile, b, mt, nt);
-        add_parts(pend_first, pend_last, -1, mt * kBM + row < p.M);
+        add_parts(pend_first, pend_last, false, mt * kBM + row < p.M);
         if (threadIdx.x == leader) counters[pend_first] = 0;
         store_out(b, mt, nt);
       }
@@ -433,21 +446,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Blocks per CTA with whole tiles, and with an equal split, which pays for joining its
-// cut tiles about as much as kSplitCost blocks take.
-constexpr int kSplitCost = 8;
+// Blocks per CTA with whole tiles, and with a split. A join takes as long as 14 blocks
+// (0.3 us each) and 3 more for a third part on: with K = 8192, 128 x 1024 takes 27.1 us
+// whole, 20.7 / 17.0 / 17.4 / 18.5 in 2 / 4 / 6 / 8 parts a tile and 28.2 on all SMs;
+// 1000 x 1000 27.9 whole, 23.1 in two, 23.8 on all; with K = 2048, 100 x 2000 9.5 whole
+// and 12.0 in two.
+constexpr JoinCost kJoin = {11, 1, 3};
 long long tiles_of(const BlockGemmArgs& L) { return L.batch * ((L.M + kBM - 1) / kBM) * ((L.N + kBN - 1) / kBN); }
 long long whole_blocks(const BlockGemmArgs& L, int sms) { return (tiles_of(L) + sms - 1) / sms * ((L.K + kBK - 1) / kBK); }
-long long split_blocks(const BlockGemmArgs& L, int sms) {
-  return (tiles_of(L) * ((L.K + kBK - 1) / kBK) + sms - 1) / sms + kSplitCost;
-}
+SplitPlan split_plan(const BlockGemmArgs& L, int sms) { return plan_split(tiles_of(L), (L.K + kBK - 1) / kBK, sms, kJoin); }
 
 }  // namespace
 
 long long block_gemm_tc_blocks(const BlockGemmArgs& L) {
   const int sms = sm_count();
   if (sms <= 0) return 0;
-  const long long w = whole_blocks(L, sms), s = split_blocks(L, sms);
+  const long long w = whole_blocks(L, sms), s = split_plan(L, sms).cost;
   return w < s ? w : s;
 }
 
@@ -467,10 +481,9 @@ int launch_block_gemm_tc(const BlockGemmArgs& L, cudaStream_t stream) {
   p.n_tiles = (p.N + kBN - 1) / kBN;
   p.tiles = L.batch * static_cast<long long>(p.m_tiles) * p.n_tiles;
   const long long total = p.tiles * p.KB;
-  p.whole = whole_blocks(L, sms) <= split_blocks(L, sms);
-  int grid = sms;
-  if (p.whole && p.tiles < grid) grid = static_cast<int>(p.tiles);
-  if (!p.whole && total < grid) grid = static_cast<int>(total);
+  const SplitPlan split = split_plan(L, sms);
+  const bool whole = whole_blocks(L, sms) <= split.cost;
+  const int grid = !whole ? split.grid : p.tiles < sms ? static_cast<int>(p.tiles) : sms;
   p.sk.total = total;
   p.sk.grid = grid;
   p.sk.kb_per_tile = p.KB;
@@ -493,14 +506,14 @@ int launch_block_gemm_tc(const BlockGemmArgs& L, cudaStream_t stream) {
                       CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != CB_OK) return st;
   constexpr size_t smem = kStages * kStageBytes + 1024;
-  static thread_local int configured_dev = -1;
+  const auto kernel = whole ? block_gemm_tc_kernel<false> : block_gemm_tc_kernel<true>;
+  static thread_local int configured_dev[2] = {-1, -1};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (configured_dev != dev) {
-    if (cudaFuncSetAttribute(block_gemm_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) !=
-        cudaSuccess)
+  if (configured_dev[whole] != dev) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
       return CB_ERR_CUDA;
-    configured_dev = dev;
+    configured_dev[whole] = dev;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -512,7 +525,7 @@ int launch_block_gemm_tc(const BlockGemmArgs& L, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, block_gemm_tc_kernel, ta, tw, p));
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, ta, tw, p));
 }
 
 }  // namespace cb
