@@ -24,7 +24,7 @@
 #include "cb_gemm_common.cuh"
 #include "cb_internal.h"
 #include "cb_ptx.cuh"
-#include "fp8_block.h"
+#include "fp8_block_out.cuh"
 
 namespace cb {
 namespace {
@@ -40,8 +40,6 @@ constexpr int kAcc = 2;
 static_assert(kStages % 2 == 0, "the two MMA issuers take alternate stages");
 constexpr uint32_t kTileBytes = 128 * kBK;            // one operand tile of one CTA
 constexpr uint32_t kStageBytes = 2 * kTileBytes;
-constexpr int kOutPitch = 80;                          // bytes of a staged row of 32 16-bit outputs
-constexpr int kOutBytes = 32 * kOutPitch;
 // Registers per thread at launch, and after the warpgroups' exchange:
 // 128 x 88 + 256 x 208 = 384 x 168.
 constexpr int kRegsLaunch = 168, kRegsFirst = 88, kRegsEpi = 208;
@@ -61,7 +59,7 @@ struct PairParams {
   void* out;
   int out_dtype;
   long long out_sb, out_sm;
-  int vec_out;
+  int unit;  // bytes of an output store
   int* status;
 };
 
@@ -132,15 +130,6 @@ __device__ __forceinline__ void tile_of(const PairParams& p, long long tile, int
   const int rows = p.m_tiles - grp * kGroupM < kGroupM ? p.m_tiles - grp * kGroupM : kGroupM;
   nt = in / rows;
   mt = grp * kGroupM + (in - nt * rows);
-}
-
-__device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
-  if (dtype == CB_DTYPE_BF16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -309,40 +298,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!live || !some) continue;
       const int n0 = nb * 128;
-      if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (n0 + i < p.N) sum[i] += load_elem(p.bias, p.bias_dtype, b * p.bias_sb + n0 + i);
-      }
-      if (p.vec_out) {
-        // 32 channels at a time through shared memory: rows of 64 bytes
-        uint16_t* out = static_cast<uint16_t*>(p.out) + b * p.out_sb;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack16(sum[c * 32 + j * 8 + 2 * i], sum[c * 32 + j * 8 + 2 * i + 1], p.out_dtype);
-            *reinterpret_cast<uint4*>(stg + lane * kOutPitch + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-          __syncwarp();
-          const int n = n0 + c * 32 + (lane & 3) * 8;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = r * 8 + (lane >> 2);
-            if (m_warp + row < p.M && n < p.N)
-              *reinterpret_cast<uint4*>(out + static_cast<long long>(m_warp + row) * p.out_sm + n) =
-                  *reinterpret_cast<const uint4*>(stg + row * kOutPitch + (lane & 3) * 16);
-          }
-          __syncwarp();
-        }
-      } else if (m < p.M) {
-        const long long orow = b * p.out_sb + static_cast<long long>(m) * p.out_sm;
-#pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (n0 + i < p.N) store_elem(p.out, p.out_dtype, orow + n0 + i, sum[i]);
-      }
+      if (p.bias) add_bias(sum, p.bias, p.bias_dtype, b * p.bias_sb + n0, p.N - n0, lane);
+      const int es = p.out_dtype == CB_DTYPE_F32 ? 4 : 2;
+      store_rows(stg, sum, static_cast<char*>(p.out) + (b * p.out_sb + static_cast<long long>(m_warp) * p.out_sm + n0) * es,
+                 p.out_sm * es, p.M - m_warp, p.N - n0, p.out_dtype, p.unit, lane);
     }
   }
 
@@ -383,8 +342,7 @@ int launch_block_gemm_pair(const BlockGemmArgs& L, cudaStream_t stream) {
   p.w_scale = L.w_scale, p.ws_sb = L.ws_sb, p.ws_sn = L.ws_sn;
   p.bias = L.bias, p.bias_dtype = L.bias_dtype, p.bias_sb = L.b_sb;
   p.out = L.out, p.out_dtype = L.out_dtype, p.out_sb = L.o_sb, p.out_sm = L.o_sm;
-  p.vec_out = (L.out_dtype == CB_DTYPE_BF16 || L.out_dtype == CB_DTYPE_F16) && L.N % 8 == 0 && aligned16(L.out) &&
-              L.o_sm % 8 == 0 && (L.batch == 1 || L.o_sb % 8 == 0);
+  p.unit = out_unit(L);
   p.status = static_cast<int*>(L.workspace);
   CUtensorMap ta, tw;
   int st = encode_tmap_3d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, L.a, L.K, L.M, L.batch, L.a_sm, L.a_sb, kBK, kBM,

@@ -29,7 +29,7 @@
 #include "cb_gemm_common.cuh"
 #include "cb_internal.h"
 #include "cb_ptx.cuh"
-#include "fp8_block.h"
+#include "fp8_block_out.cuh"
 
 namespace cb {
 namespace {
@@ -40,7 +40,7 @@ constexpr int kAcc = 4;  // accumulators in tensor memory, one per MMA issuer
 constexpr int kThreads = 512;
 // Registers: 512 x 128 at launch = 256 x 80 + 256 x 176. The epilogue holds 64 totals and
 // an accumulator's 64 columns, or two parts' quarters in flight.
-constexpr int kRegsFirst = 80, kRegsEpi = 176;
+constexpr int kRegsLaunch = 128, kRegsFirst = 80, kRegsEpi = 176;
 constexpr int kTC = 64;  // channels per epilogue warpgroup
 constexpr int kHandBar = 2, kHandThreads = 32 + 256;
 constexpr int kGroupM = 16;  // m-tiles that neighbouring CTAs share weight tiles over
@@ -61,7 +61,7 @@ struct TcParams {
   void* out;
   int out_dtype;
   long long out_sb, out_sm;
-  int vec_out;  // 16-bit output with 16-byte aligned rows, N % 8 == 0
+  int unit;  // bytes of an output store
   float* partials;  // [grid][2][kBN][kBM]
   int* counters;
   int* status;
@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       cc_z = cut_contributors(p.sk.total, p.sk.grid, p.KB, (p.sk.start(blockIdx.x + 1) - 1) / p.KB);
     }
     pdl_wait_primary();
+    uint8_t* const stg = smem + kStages * kStageBytes + (warp - 4) * kOutBytes;
     float sum[kTC];
     // Part of CTA c of a cut tile: slot 1 where the tile is cut by the end of c's range
     // (its first contributor), 0 where c's range began inside it. Token fastest.
@@ -288,44 +289,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     auto store_out = [&](int b, int mt, int nt) {
-      const int m = mt * kBM + row, n0 = nt * kBN + group * kTC;
-      if (m >= p.M || n0 >= p.N) return;
-      const long long at = b * p.out_sb + static_cast<long long>(m) * p.out_sm + n0;
-      if (p.bias) {
-#pragma unroll
-        for (int x = 0; x < kTC; ++x)
-          if (n0 + x < p.N) sum[x] += load_elem(p.bias, p.bias_dtype, b * p.bias_sb + n0 + x);
-      }
-      auto put = [&](auto* out, auto cvt) {
-        out += at;
-        bool done = false;
-        if constexpr (sizeof(*out) == 2) {
-          done = p.vec_out != 0;
-          if (done) {
-#pragma unroll
-            for (int x = 0; x < kTC; x += 8) {
-              if (n0 + x < p.N) {
-                uint4 v;
-                auto* e = reinterpret_cast<decltype(out)>(&v);
-#pragma unroll
-                for (int y = 0; y < 8; ++y) e[y] = cvt(sum[x + y]);
-                *reinterpret_cast<uint4*>(out + x) = v;
-              }
-            }
-          }
-        }
-        if (!done) {
-#pragma unroll
-          for (int x = 0; x < kTC; ++x)
-            if (n0 + x < p.N) out[x] = cvt(sum[x]);
-        }
-      };
-      if (p.out_dtype == CB_DTYPE_BF16)
-        put(static_cast<__nv_bfloat16*>(p.out), [](float v) { return __float2bfloat16_rn(v); });
-      else if (p.out_dtype == CB_DTYPE_F16)
-        put(static_cast<__half*>(p.out), [](float v) { return __float2half_rn(v); });
-      else
-        put(static_cast<float*>(p.out), [](float v) { return v; });
+      const int m0 = mt * kBM + quarter * 32, n0 = nt * kBN + group * kTC;
+      if (m0 >= p.M || n0 >= p.N) return;
+      if (p.bias) add_bias(sum, p.bias, p.bias_dtype, b * p.bias_sb + n0, p.N - n0, lane);
+      const int es = p.out_dtype == CB_DTYPE_F32 ? 4 : 2;
+      store_rows(stg, sum, static_cast<char*>(p.out) + (b * p.out_sb + static_cast<long long>(m0) * p.out_sm + n0) * es, p.out_sm * es,
+                 p.M - m0, p.N - n0, p.out_dtype, p.unit, lane);
     };
     // After an expired wait the work is skipped, but every named barrier of a group is
     // still reached by all of its warps.
@@ -492,8 +461,7 @@ int launch_block_gemm_tc(const BlockGemmArgs& L, cudaStream_t stream) {
   p.w_scale = L.w_scale, p.ws_sb = L.ws_sb, p.ws_sn = L.ws_sn;
   p.bias = L.bias, p.bias_dtype = L.bias_dtype, p.bias_sb = L.b_sb;
   p.out = L.out, p.out_dtype = L.out_dtype, p.out_sb = L.o_sb, p.out_sm = L.o_sm;
-  p.vec_out = (L.out_dtype == CB_DTYPE_BF16 || L.out_dtype == CB_DTYPE_F16) && L.N % 8 == 0 && aligned16(L.out) &&
-              L.o_sm % 8 == 0 && (L.batch == 1 || L.o_sb % 8 == 0);
+  p.unit = out_unit(L);
   Workspace ws = carve_workspace(L.workspace, grid);
   p.partials = static_cast<float*>(ws.partials);
   p.counters = ws.counters;
@@ -505,12 +473,16 @@ int launch_block_gemm_tc(const BlockGemmArgs& L, cudaStream_t stream) {
   st = encode_tmap_3d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, L.w, L.K, L.N, L.batch, L.w_sn, L.w_sb, kBK, kBN,
                       CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != CB_OK) return st;
-  constexpr size_t smem = kStages * kStageBytes + 1024;
+  constexpr size_t smem = kStages * kStageBytes + 8 * kOutBytes + 1024;
   const auto kernel = whole ? block_gemm_tc_kernel<false> : block_gemm_tc_kernel<true>;
   static thread_local int configured_dev[2] = {-1, -1};
   int dev = 0;
   cudaGetDevice(&dev);
   if (configured_dev[whole] != dev) {
+    // the warpgroups' register exchange counts on the launch's registers
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return CB_ERR_CUDA;
+    if (attr.numRegs != kRegsLaunch) return CB_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
       return CB_ERR_CUDA;
     configured_dev[whole] = dev;

@@ -107,6 +107,23 @@ def test_many_tiles(cuda_device, B, M, N, K, out_dtype):
     assert ops.device_status(cuda_device) == 0
 
 
+@pytest.mark.parametrize("M,N,K", [(100, 333, 272), (300, 1001, 2064), (1300, 2049, 272), (1300, 2050, 272)])
+@pytest.mark.parametrize("shift,pad", [(0, 0), (1, 1), (2, 6), (8, 8)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_output_rows_of_any_alignment(cuda_device, M, N, K, shift, pad, out_dtype):
+    """out starts `shift` elements into its storage, its rows N + pad apart; what lies between them is not touched."""
+    from cb200 import ops
+    a, w, a_s, w_s = _squeeze(1, *_make(1, M, N, K, M + N))
+    store = torch.full((shift + M * (N + pad),), 7.0, dtype=out_dtype, device=cuda_device)
+    out = store.as_strided((M, N), (N + pad, 1), shift)
+    ops.fp8_block_gemm(*(t.to(cuda_device) for t in (a, w, a_s, w_s)), out=out)
+    _close(out, *_exact(a, w, a_s, w_s))
+    assert torch.all(store[:shift] == 7.0)
+    if pad:
+        gaps = store[shift:].view(M, N + pad)[:, N:]
+        assert torch.all(gaps == 7.0)
+
+
 @pytest.mark.parametrize("M", [1, 3, 20, 150])
 def test_batches_and_strides(cuda_device, M):
     from cb200 import ops
