@@ -19,10 +19,11 @@ constexpr int kBlk = 128;
 
 int launch_block_gemm(const BlockGemmArgs& L, cudaStream_t stream) {
   if (L.M <= 64) return launch_block_gemm_decode(L, stream);
-  // A 256 x 256 block of a pair takes about 0.66 us, a 128 x 128 block of a CTA 0.5 us
-  // when all SMs are busy (M x N x K = 512 x 8192 x 8192: 47 us against 73 us;
-  // 256 x 8192 x 8192: 46 us against 36 us).
-  if (4 * block_gemm_pair_blocks(L) < 3 * block_gemm_tc_blocks(L)) return launch_block_gemm_pair(L, stream);
+  // A 256 x 256 block of a pair takes about 0.65 us, a 128 x 128 block of a CTA 0.45 us
+  // when all SMs are busy (M x N x K = 512 x 8192 x 8192: 45 us against 58 us; 1500 x
+  // 3000 x 6000: 38 against 66; 300 x 17408 x 5120: 56 against 54; 256 x 8192 x 8192:
+  // 43 against 33).
+  if (3 * block_gemm_pair_blocks(L) < 2 * block_gemm_tc_blocks(L)) return launch_block_gemm_pair(L, stream);
   return launch_block_gemm_tc(L, stream);
 }
 

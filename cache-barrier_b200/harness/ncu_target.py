@@ -28,13 +28,17 @@ from cb200 import ops  # noqa: E402
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--op", choices=["w8a8", "w8a8_dynamic", "fp8", "w4a16", "nvfp4", "mla"], default="w8a8")
+    ap.add_argument("--op", choices=["w8a8", "w8a8_dynamic", "fp8", "w4a16", "nvfp4", "mla", "fp8_block", "norm_block",
+                                     "paged_append", "paged_attention"], default="w8a8")
     ap.add_argument("--heads", type=int, default=16, help="mla: batch of heads (latents [heads, tokens, k])")
     ap.add_argument("--batch", type=int, default=1,
                     help="w8a8: batch of GEMMs (the reference's gate shapes: --batch 128 --k 128 --n 32*W)")
     ap.add_argument("--tokens", type=int, default=32)
     ap.add_argument("--k", type=int, default=8192)
     ap.add_argument("--n", type=int, default=8192)
+    ap.add_argument("--context", type=int, default=8192, help="paged_attention: tokens held by each of --tokens sequences")
+    ap.add_argument("--kv_heads", type=int, default=8, help="paged operators: heads of 128 (five queries each)")
+    ap.add_argument("--cache", choices=["bf16", "e4m3"], default="bf16", help="paged operators: the cache's type")
     ap.add_argument("--copies", type=int, default=4)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--launches", type=int, default=3)
@@ -99,6 +103,45 @@ def main():
         def run(i):
             qw, sw, alpha = weights[i % args.copies]
             ops.nvfp4_gemm(qa, sa, qw, sw, alpha, out=out)
+    elif args.op == "fp8_block":
+        qa, sa = ops.quant_act_fp8_block(a)
+        sw = (torch.rand(-(-N // 128), -(-K // 128), generator=g, device=dev) + 0.5) * 1e-3
+        weights = [(50 * torch.randn(N, K, generator=g, device=dev)).clamp(-448, 448).to(torch.float8_e4m3fn)
+                   for _ in range(args.copies)]
+
+        def run(i):
+            ops.fp8_block_gemm(qa, weights[i % args.copies], sa, sw, out=out)
+    elif args.op == "norm_block":
+        res, w = torch.randn_like(a), torch.ones(K, dtype=torch.bfloat16, device=dev)
+        q, s, h = ops.add_rmsnorm_quant(a, w, 1e-6, res, mode="fp8_block")
+
+        def run(i):
+            ops.add_rmsnorm_quant(a, w, 1e-6, res, mode="fp8_block", q=q, s=s, h=h)
+    elif args.op in ("paged_append", "paged_attention"):
+        Hk, D, page = args.kv_heads, 128, 64
+        ctx = args.context if args.op == "paged_attention" else 1
+        per = -(-ctx // page)
+        pages = T * per if args.op == "paged_attention" else -(-T // page)
+        shape = (pages, page, Hk, D)
+        ck, cv = (torch.randn(shape, generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2))
+        scale = None
+        if args.cache == "e4m3":
+            ck, cv = (c.to(torch.float8_e4m3fn) for c in (ck, cv))
+            scale = torch.ones(Hk, device=dev)
+        table = torch.randperm(pages, generator=torch.Generator().manual_seed(0)).to(torch.int32).to(dev)
+        if args.op == "paged_append":
+            kn, vn = (torch.randn(T, Hk, D, generator=g, device=dev).to(torch.bfloat16) for _ in range(2))
+            slots = torch.arange(T, device=dev)
+
+            def run(i):
+                ops.paged_kv_append(kn, vn, ck, cv, slots, scale, scale)
+        else:
+            qn = torch.randn(T, 5 * Hk, D, generator=g, device=dev).to(torch.bfloat16)
+            lens = torch.full((T,), ctx, dtype=torch.int32, device=dev)
+            table, o = table.view(T, per), torch.empty_like(qn)
+
+            def run(i):
+                ops.paged_decode_attention(qn, ck, cv, table, lens, k_scale=scale, v_scale=scale, out=o)
     else:
         sc = ((torch.randn(K // 128, N, generator=g, device=dev) * 0.02).abs() / 7 + 1e-4).to(torch.bfloat16)
         weights = [ops.repack_w4(torch.randint(0, 256, (K // 2, N), generator=g, dtype=torch.uint8, device=dev),
