@@ -41,6 +41,11 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
+// What a group is divided by: zeros (a padded row, or threads past a row's end) stay zeros
+// whatever it is, and 1 spares them the division proper that a step of 2^-100 takes
+// (8192 rows of 2816, whose last warp is half empty: 46 us with it).
+__device__ __forceinline__ float divisor(float amax, float step) { return amax == 0.0f ? 1.0f : step; }
+
 struct NormParams {
   const void* x;
   const void* residual;  // optional
@@ -55,41 +60,82 @@ struct NormParams {
   int int8;  // row-scale form: 1 int8, 0 e4m3
 };
 
-// Eight elements at index `at` of a row as fp32; zeros from `n` on.
+// Eight 16-bit elements at p, in the widest pieces that its address allows.
+__device__ __forceinline__ uint4 load_raw8(const uint16_t* p) {
+  const unsigned a = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p));
+  uint4 r;
+  if ((a & 15) == 0) return *reinterpret_cast<const uint4*>(p);
+  if ((a & 7) == 0) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p), y = *reinterpret_cast<const uint2*>(p + 4);
+    r = make_uint4(x.x, x.y, y.x, y.y);
+  } else if ((a & 3) == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p + 1);
+    const uint32_t first = p[0], x = w[0], y = w[1], z = w[2], last = p[7];
+    r = make_uint4(first | x << 16, x >> 16 | y << 16, y >> 16 | z << 16, z >> 16 | last << 16);
+  }
+  return r;
+}
+
+__device__ __forceinline__ void store_raw8(uint16_t* p, uint4 r) {
+  const unsigned a = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p));
+  if ((a & 15) == 0) {
+    *reinterpret_cast<uint4*>(p) = r;
+  } else if ((a & 7) == 0) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(r.x, r.y);
+    *reinterpret_cast<uint2*>(p + 4) = make_uint2(r.z, r.w);
+  } else if ((a & 3) == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(p);
+    w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(p + 1);
+    p[0] = static_cast<uint16_t>(r.x);
+    w[0] = r.x >> 16 | r.y << 16, w[1] = r.y >> 16 | r.z << 16, w[2] = r.z >> 16 | r.w << 16;
+    p[7] = static_cast<uint16_t>(r.w >> 16);
+  }
+}
+
+// Eight elements at index `at` of a row as fp32; zeros from `n` on. VEC: rows are whole
+// 16-byte vectors; else in pieces (element by element, rows of 8404 took 52 us for 1310).
 template <bool VEC, typename T>
 __device__ __forceinline__ void load8(const T* row, int at, int n, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (at < n) {
-      if constexpr (sizeof(T) == 2) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(row + at);
-        const T* e = reinterpret_cast<const T*>(&raw);
+  if (at + 8 <= n || (VEC && at < n)) {
+    if constexpr (sizeof(T) == 2) {
+      uint4 raw;
+      if constexpr (VEC)
+        raw = *reinterpret_cast<const uint4*>(row + at);
+      else
+        raw = load_raw8(reinterpret_cast<const uint16_t*>(row + at));
+      const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
-      } else {
-        const float4 a = *reinterpret_cast<const float4*>(row + at), b = *reinterpret_cast<const float4*>(row + at + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      }
-      return;
+      for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+    } else if (VEC || (reinterpret_cast<uintptr_t>(row + at) & 15) == 0) {
+      const float4 a = *reinterpret_cast<const float4*>(row + at), b = *reinterpret_cast<const float4*>(row + at + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_f32(row[at + j]);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = at + j < n ? to_f32(row[at + j]) : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = !VEC && at + j < n ? to_f32(row[at + j]) : 0.0f;
   }
 }
 
 template <bool VEC, typename T>
 __device__ __forceinline__ void store8(T* row, int at, int n, const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (at < n) {
-      uint4 raw;
-      T* e = reinterpret_cast<T*>(&raw);
+  if (at + 8 <= n || (VEC && at < n)) {
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) from_f32(v[j], e[j]);
+    for (int j = 0; j < 8; ++j) from_f32(v[j], e[j]);
+    if constexpr (VEC)
       *reinterpret_cast<uint4*>(row + at) = raw;
-    }
-  } else {
+    else
+      store_raw8(reinterpret_cast<uint16_t*>(row + at), raw);
+  } else if constexpr (!VEC) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (at + j < n) from_f32(v[j], row[at + j]);
@@ -98,12 +144,31 @@ __device__ __forceinline__ void store8(T* row, int at, int n, const float (&v)[8
 
 template <bool VEC>
 __device__ __forceinline__ void store_q8(uint8_t* row, int at, int n, uint64_t q) {
+  uint8_t* const p = row + at;
   if constexpr (VEC) {
-    if (at < n) *reinterpret_cast<uint64_t*>(row + at) = q;
+    if (at < n) *reinterpret_cast<uint64_t*>(p) = q;
+  } else if (at + 8 <= n) {
+    const unsigned a = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p));
+    const uint32_t lo = static_cast<uint32_t>(q), hi = static_cast<uint32_t>(q >> 32);
+    if ((a & 7) == 0) {
+      *reinterpret_cast<uint64_t*>(p) = q;
+    } else if ((a & 3) == 0) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(p);
+      w[0] = lo, w[1] = hi;
+    } else if ((a & 1) == 0) {
+      uint16_t* w = reinterpret_cast<uint16_t*>(p);
+      w[0] = static_cast<uint16_t>(lo), w[1] = static_cast<uint16_t>(lo >> 16);
+      w[2] = static_cast<uint16_t>(hi), w[3] = static_cast<uint16_t>(hi >> 16);
+    } else {
+      uint16_t* w = reinterpret_cast<uint16_t*>(p + 1);
+      p[0] = static_cast<uint8_t>(lo);
+      w[0] = static_cast<uint16_t>(lo >> 8), w[1] = static_cast<uint16_t>(q >> 24), w[2] = static_cast<uint16_t>(hi >> 8);
+      p[7] = static_cast<uint8_t>(hi >> 24);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (at + j < n) row[at + j] = static_cast<uint8_t>(q >> (8 * j));
+      if (at + j < n) p[j] = static_cast<uint8_t>(q >> (8 * j));
   }
 }
 
@@ -189,8 +254,9 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormParams p) {
     float step[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      step[v] = fmaxf(__fdiv_rn(group_max(amax8(u[v])), 448.0f), kNormFloor);
-      store_q8<VEC>(q, (v * blockDim.x + threadIdx.x) * 8, p.H, quant8<false>(u[v], step[v]));
+      amax = group_max(amax8(u[v]));
+      step[v] = fmaxf(__fdiv_rn(amax, 448.0f), kNormFloor);
+      store_q8<VEC>(q, (v * blockDim.x + threadIdx.x) * 8, p.H, quant8<false>(u[v], divisor(amax, step[v])));
     }
     row_sum_max(ss, amax, red);
     const float r = row_factor(ss, p.H, p.eps);
@@ -205,11 +271,11 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormParams p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) amax = fmaxf(amax, amax8(u[v]));
     row_sum_max(ss, amax, red);
-    const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor);
+    const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor), div = divisor(amax, step);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       store_q8<VEC>(q, (v * blockDim.x + threadIdx.x) * 8, p.H,
-                    p.int8 ? quant8<true>(u[v], step) : quant8<false>(u[v], step));
+                    p.int8 ? quant8<true>(u[v], div) : quant8<false>(u[v], div));
     if (threadIdx.x == 0) p.scale[row * p.s_sm] = __fmul_rn(step, row_factor(ss, p.H, p.eps));
   }
 }
@@ -290,8 +356,9 @@ __global__ void __launch_bounds__(512, NV == 4 ? 1 : 2) norm_rows_kernel(const N
       float step[NV];
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        step[v] = fmaxf(__fdiv_rn(group_max(amax8(u[v])), 448.0f), kNormFloor);
-        store_q8<true>(q, (v * n + tid) * 8, p.H, quant8<false>(u[v], step[v]));
+        amax = group_max(amax8(u[v]));
+        step[v] = fmaxf(__fdiv_rn(amax, 448.0f), kNormFloor);
+        store_q8<true>(q, (v * n + tid) * 8, p.H, quant8<false>(u[v], divisor(amax, step[v])));
       }
       row_sum_max(ss, amax, red[parity]);
       const float r = row_factor(ss, p.H, p.eps);
@@ -306,10 +373,10 @@ __global__ void __launch_bounds__(512, NV == 4 ? 1 : 2) norm_rows_kernel(const N
 #pragma unroll
       for (int v = 0; v < NV; ++v) amax = fmaxf(amax, amax8(u[v]));
       row_sum_max(ss, amax, red[parity]);
-      const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor);
+      const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor), div = divisor(amax, step);
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        store_q8<true>(q, (v * n + tid) * 8, p.H, p.int8 ? quant8<true>(u[v], step) : quant8<false>(u[v], step));
+        store_q8<true>(q, (v * n + tid) * 8, p.H, p.int8 ? quant8<true>(u[v], div) : quant8<false>(u[v], div));
       if (tid == 0) p.scale[row * p.s_sm] = __fmul_rn(step, row_factor(ss, p.H, p.eps));
     }
     stage = stage == AHEAD ? 0 : stage + 1;
@@ -356,8 +423,9 @@ __global__ void __launch_bounds__(kMaxThreads) norm_long_kernel(const NormParams
     const int at = at64 < p.H ? static_cast<int>(at64) : p.H;
     weighted(at, u, &ss);
     if constexpr (BLOCK) {
-      const float step = fmaxf(__fdiv_rn(group_max(amax8(u)), 448.0f), kNormFloor);
-      store_q8<false>(q, at, p.H, quant8<false>(u, step));
+      amax = group_max(amax8(u));
+      const float step = fmaxf(__fdiv_rn(amax, 448.0f), kNormFloor);
+      store_q8<false>(q, at, p.H, quant8<false>(u, divisor(amax, step)));
       if ((threadIdx.x & 15) == 0 && at < p.H) p.scale[row * p.s_sm + at / kGroup] = step;  // times r below
     } else {
       amax = fmaxf(amax, amax8(u));
@@ -371,12 +439,12 @@ __global__ void __launch_bounds__(kMaxThreads) norm_long_kernel(const NormParams
       if ((threadIdx.x & 15) == 0 && at < p.H) p.scale[row * p.s_sm + at / kGroup] *= r;
     }
   } else {
-    const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor);
+    const float step = fmaxf(__fdiv_rn(amax, p.int8 ? 127.0f : 448.0f), kNormFloor), div = divisor(amax, step);
     for (long long base = 0; base < p.H; base += span) {
       const long long at = base + threadIdx.x * 8;
       if (at >= p.H) break;
       weighted(static_cast<int>(at), u, nullptr);
-      store_q8<false>(q, static_cast<int>(at), p.H, p.int8 ? quant8<true>(u, step) : quant8<false>(u, step));
+      store_q8<false>(q, static_cast<int>(at), p.H, p.int8 ? quant8<true>(u, div) : quant8<false>(u, div));
     }
     if (threadIdx.x == 0) p.scale[row * p.s_sm] = __fmul_rn(step, r);
   }
@@ -441,7 +509,7 @@ int launch_norm(const NormParams& p, bool vec, cudaStream_t stream) {
   if (vec) {
     if (warp_rows)
       nv = vecs <= 32 ? 1 : vecs <= 64 ? 2 : 4;
-    else if (p.rows <= 2 * 148)
+    else if (p.rows <= 2LL * sm_count())
       nv = vecs <= kMaxThreads ? 1 : vecs <= 2 * kMaxThreads ? 2 : 4;
   }
   const int per = (vecs + nv - 1) / nv;
