@@ -16,9 +16,10 @@
 //
 // CTAs take whole tiles, or, where that leaves SMs idle, the k-blocks of all tiles end
 // to end in one contiguous range per CTA (cb_gemm_common.cuh), as many CTAs as pay for
-// the join (plan_split): parts of a cut tile are published as they end, and the tile's first contributor adds them in CTA order after
-// a short bounded poll, else the last to arrive does. No CTA waits for one that may
-// not run, and the bits do not depend on who adds.
+// the join (plan_split): parts of a cut tile are published as they end, and the tile's
+// first contributor adds them in CTA order after a short bounded poll, else the last to
+// arrive does. No CTA waits for one that may not run, and the bits do not depend on who
+// adds.
 //
 // Warps: 0, 12 TMA producers; 1-3, 13 MMA issuers; 14-15 accumulator waiters; 4-11
 // epilogue.
