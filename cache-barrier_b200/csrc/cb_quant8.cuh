@@ -2,14 +2,23 @@
 // fp32 quotient.
 //
 // The eight quotients share a divisor, so they come from its reciprocal: with
-// y = RN(1 / step), q0 = RN(u y) and the remainder r = u - q0 step by a fused
-// multiply-add, RN(q0 + r y) is the correctly rounded quotient (P. Markstein,
-// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990,
-// theorem 8, where q0 is within a unit in the last place; one beyond that is off by
-// 1e-7 units before its rounding, which no 8-bit boundary tells apart in practice).
+// y = RN(1 / step), q = RN(u y) and the remainder r = q step - u by a fused
+// multiply-add, RN(q - r y) is the correctly rounded quotient where q is within a unit in
+// the last place (P. Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990, theorem 8). q may be up to 1.5 units off, and r then
+// rounds too: before its own rounding the result is within 2^-22 units of u / step. So
+// the 8-bit result can differ from that of a division only where u / step is that close
+// to the midpoint between a tie of the 8-bit type and the next fp32 value. For e4m3 and
+// 16-bit u that leaves one family, step = (1 - 2^-24) 2^n under a power of two, which comes
+// out right (the test of the append holds all 16-bit u against 4096 divisors); the norm's
+// fp32 u have no such bound and may round the other way there.
 // Three instructions a value; an IEEE division each (about 20) made the kernels that
-// use this issue-bound. Steps whose reciprocal or remainder would leave the normal
-// range (below 2^-60, above 2^126, NaN) are divided.
+// use this issue-bound. The remainder is taken with its sign turned, so that a zero
+// quotient keeps its sign. Steps whose reciprocal or remainder would leave the normal
+// range (below 2^-60, above 2^126, NaN) are divided, and so, unless BOUNDED, are eight
+// values of which one is beyond 512 steps: where q is infinite, q - r y is not a number.
+// BOUNDED says that no value exceeds 512 steps (steps that come from the values' own
+// maximum; an infinity there makes the step infinite).
 #pragma once
 
 #include <cstdint>
@@ -18,17 +27,25 @@
 namespace cb {
 
 // int8 rounds half away from zero, e4m3 to nearest even, saturated.
-template <bool INT8>
+template <bool INT8, bool BOUNDED = true>
 __device__ __forceinline__ uint64_t quant8(const float (&u)[8], float step) {
   float v[8];
-  if (step >= 8.673617379884035e-19f && step <= 8.507059173023462e+37f) {  // 2^-60, 2^126
+  bool multiply = step >= 8.673617379884035e-19f && step <= 8.507059173023462e+37f;  // 2^-60, 2^126
+  if (multiply) {
     const float y = __fdiv_rn(1.0f, step);
+    float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float q = __fmul_rn(u[j], y);
-      v[j] = __fmaf_rn(__fmaf_rn(-q, step, u[j]), y, q);
+      v[j] = __fmul_rn(u[j], y);
+      if constexpr (!BOUNDED) top = fmaxf(top, fabsf(v[j]));  // NaN: stays NaN either way
     }
-  } else {
+    if constexpr (!BOUNDED) multiply = top < 512.0f;
+    if (multiply) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __fmaf_rn(-__fmaf_rn(v[j], step, -u[j]), y, v[j]);
+    }
+  }
+  if (!multiply) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(u[j], step);
   }

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
           float u[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) u[j] = to_f32(e[j]);
-          const uint64_t q = quant8<false>(u, scale);
+          const uint64_t q = quant8<false, false>(u, scale);  // keys are not bounded by their scale
           out = *reinterpret_cast<const Out*>(&q);
         } else {
 #pragma unroll
