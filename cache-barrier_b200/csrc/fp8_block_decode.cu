@@ -73,6 +73,7 @@ struct DecodeParams {
   float* partials;    // [grid][2][TN][128]
   int* counters;
   int* status;
+  unsigned long long dbg_wait_ns;  // failure-detection test hook: limit of a wait that expires (0: off)
 };
 
 // A unit's place, advanced without division.
@@ -194,7 +195,8 @@ __global__ void __launch_bounds__(kThreads<TN>, kPerSm<TN>)
       const uint32_t idesc = idesc_e4m3_f32(kBlk, TN);
       int stage = j;
       uint32_t phase = 0;
-      for (; i < units; i += 2) {
+      const bool dead = j == 0 && p.dbg_wait_ns != 0 && !wait_counter(p.status + 1, 1, abort_ptr, p.status, p.dbg_wait_ns);
+      for (; i < units && !dead; i += 2) {
         const int acc = i % kAcc;
         if (!mbar_wait_quick(&tempty_bar[acc], static_cast<uint32_t>((i / kAcc) & 1) ^ 1u, abort_ptr, p.status) ||
             !mbar_wait_quick(&full_bar[stage], phase, abort_ptr, p.status))
@@ -260,7 +262,8 @@ __global__ void __launch_bounds__(kThreads<TN>, kPerSm<TN>)
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + group * TC;
     const int M = p.M - group * TC < TC ? p.M - group * TC : TC;  // this group's tokens (none: it only keeps the barriers)
     // After an expired wait the work is skipped, but every named barrier of a group is
-    // still reached by all of its warps.
+    // still reached by all of its warps, and the hand-over barriers until both waiters
+    // have left.
     bool live = true;
     Unit u = steady;
     int i = 0;
@@ -345,7 +348,11 @@ __global__ void __launch_bounds__(kThreads<TN>, kPerSm<TN>)
       for (int k = 0; k < here && live; ++k) {
         const int n = i + k, acc = n % kAcc;
         live = !named_bar_or(kHandBar + (n & 1), kHandThreads, false);
-        if (!live) break;
+        if (!live) {
+          // the other waiter comes to the next unit's barrier, whatever it has seen: it leaves from there
+          if (n + 1 < units) named_bar_or(kHandBar + ((n + 1) & 1), kHandThreads, true);
+          break;
+        }
         tc_fence_after();
         uint32_t r[TC / 16][16];
 #pragma unroll
@@ -507,6 +514,7 @@ int launch_block_gemm_decode(const BlockGemmArgs& L, cudaStream_t stream) {
   p.bias = L.bias, p.bias_dtype = L.bias_dtype, p.bias_sb = L.b_sb;
   p.out = L.out, p.out_dtype = L.out_dtype, p.out_sb = L.o_sb, p.out_sm = L.o_sm;
   p.sk.first_poll_ns = debug_force_last_arriver() ? 0 : kFirstPollNs;
+  p.dbg_wait_ns = debug_wait_ns();
   Workspace ws = carve_workspace(L.workspace, grid);
   p.partials = static_cast<float*>(ws.partials);
   p.counters = ws.counters;

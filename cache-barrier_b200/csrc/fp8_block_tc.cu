@@ -66,6 +66,7 @@ struct TcParams {
   float* partials;  // [grid][2][kBN][kBM]
   int* counters;
   int* status;
+  unsigned long long dbg_wait_ns;  // failure-detection test hook: limit of a wait that expires (0: off)
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -201,7 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int i = j;
       if (lane == 0) {
         const uint32_t idesc = idesc_e4m3_f32(kBM, kBN);
-        for (; i < units; i += kAcc) {
+        const bool dead = j == 0 && p.dbg_wait_ns != 0 && !wait_counter(p.status + 1, 1, abort_ptr, p.status, p.dbg_wait_ns);
+        for (; i < units && !dead; i += kAcc) {
           const int stage = i % kStages;
           if (!mbar_wait_quick(&tempty_bar[j], static_cast<uint32_t>((i / kAcc) & 1) ^ 1u, abort_ptr, p.status) ||
               !mbar_wait_quick(&full_bar[stage], static_cast<uint32_t>((i / kStages) & 1), abort_ptr, p.status))
@@ -218,7 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(&drain_bar[j]);
       }
       // Every commit's arrival must land before the CTA exits: the MMAs' end, the last
-      // use of each stage (waited for by the warp that issued it) and the last hand-off.
+      // use of each stage (waited for by the warp that issued it; after an expired wait at
+      // the end, when all know what was issued) and the last hand-off.
       i = __shfl_sync(0xffffffffu, i, 0);
       if (lane == 31) mbar_wait_quick(&drain_bar[j], 0, nullptr, p.status);
       const int js = i - kAcc - kAcc * lane;
@@ -298,7 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                  p.M - m0, p.N - n0, p.out_dtype, p.unit, lane);
     };
     // After an expired wait the work is skipped, but every named barrier of a group is
-    // still reached by all of its warps.
+    // still reached by all of its warps, and the hand-over barriers until both waiters
+    // have left.
     bool live = true;
     // Stores this CTA's part; after the barrier the leader's fence covers all of them.
     auto publish = [&](int c_first, bool row_live) {
@@ -329,7 +333,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float f = row_live ? next : 0.0f;
         if (k + 1 < here) next = __ldg(as + k + 1) * __ldg(ws + k + 1);
         live = !named_bar_or(kHandBar + (n & 1), kHandThreads, false);
-        if (!live) break;
+        if (!live) {
+          // the other waiter comes to the next unit's barrier, whatever it has seen: it leaves from there
+          if (n + 1 < units) named_bar_or(kHandBar + ((n + 1) & 1), kHandThreads, true);
+          break;
+        }
         if (some) {
           tc_fence_after();
           uint32_t r[2][32];
@@ -401,6 +409,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   __syncthreads();
   if (warp == 0) {
+    if (abort_flag && lane < kStages) {
+      // the last use of stage `lane`: unit k of issuer j, the stage again every 3 of its units
+      int last = -1;
+      for (int j = 0; j < kAcc; ++j)
+        for (int x = 1, k = sh_consumed[j] - kAcc; x <= kStages / 2 && k >= 0; ++x, k -= kAcc)
+          if (k % kStages == lane && k > last) last = k;
+      if (last >= 0) mbar_wait_quick(&empty_bar[lane], static_cast<uint32_t>((last / kStages) & 1), nullptr, p.status);
+    }
+    __syncwarp();
     if (lane == 0 && abort_flag) {
       // loads issued but never consumed must land before the CTA exits
       for (int j = 0; j < kAcc; ++j)
@@ -458,6 +475,7 @@ int launch_block_gemm_tc(const BlockGemmArgs& L, cudaStream_t stream) {
   p.sk.grid = grid;
   p.sk.kb_per_tile = p.KB;
   p.sk.first_poll_ns = debug_force_last_arriver() ? 0 : kFirstPollNs;
+  p.dbg_wait_ns = debug_wait_ns();
   p.a_scale = L.a_scale, p.as_sb = L.as_sb, p.as_sm = L.as_sm;
   p.w_scale = L.w_scale, p.ws_sb = L.ws_sb, p.ws_sn = L.ws_sn;
   p.bias = L.bias, p.bias_dtype = L.bias_dtype, p.bias_sb = L.b_sb;

@@ -117,14 +117,15 @@ CB_API int cb_workspace_status(void* workspace, int* device_status, cb_stream_t 
 
 /* Failure-detection test hook (no counterpart in the reference). With a
    nonzero limit_ns, every later W8A8 GEMM launch (all W8A8 entry points and
-   the W4A4 path) makes one epilogue thread per CTA wait, bounded by limit_ns,
-   on a workspace word that nothing sets: the wait expires, the kernel records
-   CB_DEVERR_TIMEOUT in its status word and every role of the CTA takes its
-   abort path (skips its remaining work, drains its copies and MMAs, frees its
-   tensor memory), so the GPU context stays usable and the caller sees the
-   timeout through cb_workspace_status / cb_w8a8_noalloc_status. The output of
-   such a call is undefined. 0 (the default) turns the hook off. Process-wide;
-   for tests only. */
+   the W4A4 path) makes one epilogue thread per CTA, and every block-scaled FP8
+   GEMM of CTAs on their own (up to 64 tokens, and 128 x 128 tiles) one thread
+   that issues MMAs, wait, bounded by limit_ns, on a workspace word that nothing
+   sets: the wait expires, the kernel records CB_DEVERR_TIMEOUT in its status
+   word and every role of the CTA takes its abort path (skips its remaining
+   work, drains its copies and MMAs, frees its tensor memory), so the GPU
+   context stays usable and the caller sees the timeout through
+   cb_workspace_status / cb_w8a8_noalloc_status. The output of such a call is
+   undefined. 0 (the default) turns the hook off. Process-wide; for tests only. */
 CB_API void cb_debug_force_wait_timeout(uint64_t limit_ns);
 
 /* Split-K test hook (no counterpart in the reference). A tile whose k-blocks
