@@ -35,7 +35,11 @@
 // The order of d inside a k-step and of the output rows is free, so a lane's
 // 16-byte loads of K (token g, d 8t..8t+7) and V (tokens 2t, 2t+1, 2t+8, 2t+9,
 // d 8g..8g+7) are the fragments after byte permutes, with no shared memory.
-// P^T is the transpose of the S^T accumulator: one movmatrix per 8 tokens. Heads
+// P^T is the transpose of the S^T accumulator: one movmatrix per 8 tokens and term. P is
+// the sum of two values of the products' 16-bit type, a leading one towards zero and what
+// that leaves, so that 2^-16 (bf16) or 2^-21 (f16) of a probability is lost, not 2^-9 or
+// 2^-12; the remainder is never zero nor negative, so an infinite value of V stays
+// infinite. Heads
 // are the narrow side (n = 8): a group of 5 to 8 wastes little and one wasted
 // column costs no bandwidth. mma.sync is enough here: at 8 heads the products
 // need a few percent of its rate at full cache bandwidth, and tcgen05 would need
@@ -131,6 +135,13 @@ struct Math<true> {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
+  // Two values >= 0 towards zero, and what that leaves of them, in the same type.
+  static __device__ __forceinline__ uint32_t split(float lo, float hi, uint32_t& rest) {
+    const uint32_t head = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+    rest = pack(fmaxf(lo - __uint_as_float(head << 16), kLeast), fmaxf(hi - __uint_as_float(head & 0xffff0000u), kLeast));
+    return head;
+  }
+  static constexpr float kLeast = 1.1754943508222875e-38f;  // 2^-126
 };
 template <>
 struct Math<false> {
@@ -145,6 +156,14 @@ struct Math<false> {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
+  static __device__ __forceinline__ uint32_t split(float lo, float hi, uint32_t& rest) {
+    uint32_t head;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(head) : "f"(hi), "f"(lo));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&head));
+    rest = pack(fmaxf(lo - v.x, kLeast), fmaxf(hi - v.y, kLeast));
+    return head;
+  }
+  static constexpr float kLeast = 5.9604644775390625e-8f;  // 2^-24, of probabilities up to 2^15
 };
 
 // Two e4m3 values (exact) as f16x2.
@@ -518,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QT, FP8, D, NT>::kMinCtas) att
         load_k(tl + 1);
       }
       // ---- running maximum and sum ----
-      uint32_t pb[NT][2];
+      uint32_t pb[NT][2], pr[NT][2];  // the probabilities' leading and remaining terms
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float x[4], mx[2];
@@ -547,8 +566,12 @@ __global__ void __launch_bounds__(kThreads, Shape<QT, FP8, D, NT>::kMinCtas) att
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][n][j] *= al[j & 1];
         }
-        pb[n][0] = movmatrix_trans(M::pack(x[0], x[1]));
-        pb[n][1] = movmatrix_trans(M::pack(x[2], x[3]));
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t rest;
+          pb[n][r] = movmatrix_trans(M::split(x[2 * r], x[2 * r + 1], rest));
+          pr[n][r] = movmatrix_trans(rest);
+        }
       }
       // ---- output ----
 #pragma unroll
@@ -567,13 +590,19 @@ __global__ void __launch_bounds__(kThreads, Shape<QT, FP8, D, NT>::kMinCtas) att
               const uint32_t a0 = e4m3x2_f16x2(lo), a1 = e4m3x2_f16x2(lo >> 16);
               const uint32_t a2 = e4m3x2_f16x2(hi), a3 = e4m3x2_f16x2(hi >> 16);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) M::mma(o[(c * (S::kVV / 4) + w) * 2 + hl][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+              for (int n = 0; n < NT; ++n) {
+                M::mma(o[(c * (S::kVV / 4) + w) * 2 + hl][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                M::mma(o[(c * (S::kVV / 4) + w) * 2 + hl][n], a0, a1, a2, a3, pr[n][0], pr[n][1]);
+              }
             }
           } else {
             const uint32_t a0 = __byte_perm(v0[w], v1[w], 0x5410), a1 = __byte_perm(v0[w], v1[w], 0x7632);
             const uint32_t a2 = __byte_perm(v2[w], v3[w], 0x5410), a3 = __byte_perm(v2[w], v3[w], 0x7632);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) M::mma(o[c * (S::kVV / 4) + w][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+            for (int n = 0; n < NT; ++n) {
+              M::mma(o[c * (S::kVV / 4) + w][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+              M::mma(o[c * (S::kVV / 4) + w][n], a0, a1, a2, a3, pr[n][0], pr[n][1]);
+            }
           }
         }
       }
