@@ -447,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, Shape<QT, FP8, D, NT>::kMinCtas) att
     }
     __syncthreads();  // the previous item is done with the shared memory
     if constexpr (S::kScaleQ) {
-      // power of two that brings each query row's largest value to [1, 2)
+      // power of two that brings each query row's largest value to [2^14, 2^15): f16 then
+      // holds values down to 2^-28 of it with all of bf16's bits
       float m = 0.0f;
 #pragma unroll
       for (int x = 0; x < kQ; ++x) {
@@ -463,10 +464,10 @@ __global__ void __launch_bounds__(kThreads, Shape<QT, FP8, D, NT>::kMinCtas) att
         float top = 0.0f;
 #pragma unroll
         for (int w = tid / 8; w < kWarps; w += NT) top = fmaxf(top, sh_qmax[w][tid % 8]);
-        int e = 0;
+        int e = 14;  // an infinite row stays as it is
         if (top > 0.0f && top < INFINITY) e = ilogbf(top);
-        if (e < -100) e = -100;  // rows below 2^-100 keep a factor that fp32 holds
-        sh_qexp[tid] = ldexpf(1.0f, e);
+        if (e < -86) e = -86;  // rows below 2^-86 keep a factor that fp32 holds
+        sh_qexp[tid] = ldexpf(1.0f, e - 14);
       }
       __syncthreads();
     }

@@ -6,6 +6,8 @@ The probabilities enter their product as a leading and a remaining term of the p
 A = sum_l p_l |v_l| and Z = max_l scale * sum_d |q_d k_d|, the scores are fp32 sums of
 exact products (2^-16 Z off at most, 256 additions), the output within
 (u + 2 dz) A of exact, dz = 2^-16 Z + 2^-20, and its own rounding comes on top.
+Queries of bf16 over an e4m3 cache become f16 beside a power of two that puts the row's
+largest value at 2^14: values down to 2^-28 of it keep all their bits.
 """
 
 import math
@@ -79,6 +81,30 @@ def test_one_key_against_its_opposite(cuda_device):
         k[0, 0, 0], v[1] = 1.0, -1.0
         k, v = k.to(cache_dtype), v.to(cache_dtype)
         _check(_run(ops, q, k, v, 16, cuda_device), q, k, v, u)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("gain", [1.0, 2.0 ** 60, 2.0 ** -60])
+def test_small_query_values_beside_a_large_one(cuda_device, D, gain):
+    """The row's largest value meets zeros; the scores come from values 2^-20 of it."""
+    from cb200 import ops
+    g = torch.Generator().manual_seed(D)
+    L, Hkv, G = 40, 2, 5
+    q = torch.randn(1, Hkv * G, D, generator=g) * 2.0 ** -20
+    q[..., 7] = 1.5
+    q = q.to(torch.bfloat16)
+    k = torch.randn(L, Hkv, D, generator=g) * 100.0
+    k[..., 7] = 0.0
+    k, v = k.to(FP8), torch.randn(L, Hkv, D, generator=g).to(FP8)
+    scale = torch.full((Hkv,), 2.0 ** 14, device=cuda_device)  # scores of about one
+    pages = -(-L // 16)
+    kc, vc = (torch.zeros(pages * 16, Hkv, D, dtype=torch.uint8) for _ in range(2))
+    kc[:L], vc[:L] = k.view(torch.uint8), v.view(torch.uint8)
+    kc, vc = (c.view(FP8).view(pages, 16, Hkv, D).to(cuda_device) for c in (kc, vc))
+    out = ops.paged_decode_attention((q.float() * gain).to(torch.bfloat16).to(cuda_device), kc, vc,
+                                     torch.arange(pages, dtype=torch.int32, device=cuda_device)[None],
+                                     torch.tensor([L], dtype=torch.int32, device=cuda_device), k_scale=scale / gain)
+    _check(out.double().cpu(), q, k.double() * 2.0 ** 14, v, 2.0 ** -21)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
