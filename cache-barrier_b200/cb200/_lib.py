@@ -90,6 +90,9 @@ SIGNATURES = {
     "cb_exec_synchronize": (_int, [_vp, ctypes.POINTER(_int)]),
     "cb_exec_w8a8_dynamic_host": (_int, [_vp, _vp, _int, _vp, _vp, _i64, _i64, _i64, _vp, _int, _i64, _i64, _i64,
                                          _i64]),
+    "cb_stream_capture_id": (ctypes.c_uint64, [_vp]),
+    "cb_capture_workspace": (_int, [_vp, _sz, ctypes.POINTER(_vp)]),
+    "cb_capture_live": (_int, [ctypes.c_uint64]),
     "cb_debug_force_wait_timeout": (None, [ctypes.c_uint64]),
     "cb_debug_force_last_arriver": (None, [ctypes.c_int]),
     "cb_w8a8_gemm_dynamic": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp,

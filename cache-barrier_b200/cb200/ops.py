@@ -56,55 +56,99 @@ def _as3d(t: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------
-# Workspace pool: one zero-initialised scratch buffer per (device, stream).
+# Workspace pool: one zero-initialised scratch buffer per (device, stream), and per
+# (device, stream, capture) inside CUDA graphs.
 # ---------------------------------------------------------------------------
+class _CapturedWorkspace:
+    """A workspace that the library holds for one graph (``cb_capture_workspace``)."""
+
+    def __init__(self, address: int, nbytes: int):
+        self._address, self._nbytes = address, nbytes
+
+    def data_ptr(self) -> int:
+        return self._address
+
+    def numel(self) -> int:
+        return self._nbytes
+
+
 class WorkspacePool:
     """Caller-owned split-K scratch for the C ABI.
 
     Buffers are zero-filled at allocation and left zeroed by the kernels. One
-    buffer per (device, stream) so concurrent streams never share scratch. A
-    buffer first needed while a CUDA graph is being captured (torch captures on
-    its own stream) is allocated from the graph's memory pool; its zero-fill is
-    captured with it and re-runs on every replay, which keeps it valid.
+    buffer per (device, stream) so concurrent streams never share scratch. While a
+    CUDA graph is being captured, one per (device, stream, capture): graphs share
+    none, with each other or with eager calls, so they may be replayed in any order
+    and at the same time. Those are the library's, outside the graph's memory pool,
+    zeroed when they are handed out, and free for a later capture once the graph is
+    gone. A buffer that a larger one replaces is kept: its status word is still read.
     """
 
     def __init__(self):
-        self._bufs = {}
+        self._bufs = {}  # (device index, stream, capture id or 0) -> [replaced .., current]
         self._lock = threading.Lock()
         self._native = None  # the native layer, once it holds addresses of these buffers
 
-    def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
-        key = (device.index, _stream(device))
+    def get(self, nbytes: int, device: torch.device):
+        """The current buffer of ``device``'s current stream, of at least ``nbytes``."""
+        stream = _stream(device)
+        key = (device.index, stream, L.load().cb_stream_capture_id(stream))
         with self._lock:
-            buf = self._bufs.get(key)
-            if buf is None or buf.numel() < nbytes:
+            held = self._bufs.get(key)
+            if held is None or held[-1].numel() < nbytes:
                 size = max(nbytes, 1 << 20)
-                if buf is not None:
-                    size = max(size, 2 * buf.numel())
-                buf = torch.zeros(size, dtype=torch.uint8, device=device)
-                self._bufs[key] = buf
+                if held is not None:
+                    size = max(size, 2 * held[-1].numel())
+                if key[2]:
+                    buf = self._captured(size, stream, device)
+                else:
+                    buf = torch.zeros(size, dtype=torch.uint8, device=device)
+                self._forget_dead()
+                held = self._bufs.setdefault(key, [])
+                held.append(buf)
                 if self._native is not None:
                     self._native.set_workspace(*key, buf.data_ptr(), buf.numel())
-            return buf
+            return held[-1]
+
+    @staticmethod
+    def _captured(size: int, stream: int, device: torch.device) -> _CapturedWorkspace:
+        p = ctypes.c_void_p()
+        with torch.cuda.device(device):
+            L.check("cb_capture_workspace", L.load().cb_capture_workspace(stream, size, ctypes.byref(p)))
+        return _CapturedWorkspace(p.value, size)
+
+    def _forget_dead(self) -> None:
+        """Drops the buffers of graphs that are gone; the library has them back."""
+        for key in [k for k in self._bufs if k[2] and not L.load().cb_capture_live(k[2])]:
+            del self._bufs[key]
+            if self._native is not None:
+                self._native.drop_workspace(*key)
 
     def share(self, nbytes: int, device: torch.device, native) -> None:
         """``get``, and the buffer's address to the native layer. That layer asks again
         where it needs more bytes; ``get`` tells it when a buffer is replaced."""
         self._native = native
         buf = self.get(nbytes, device)
-        native.set_workspace(device.index, _stream(device), buf.data_ptr(), buf.numel())
+        stream = _stream(device)
+        native.set_workspace(device.index, stream, L.load().cb_stream_capture_id(stream), buf.data_ptr(), buf.numel())
 
     def check_status(self, device: torch.device | None = None) -> int:
         """Synchronising read of the device status word of every buffer on device."""
         worst = 0
-        for (idx, stream), buf in list(self._bufs.items()):
+        with self._lock:
+            self._forget_dead()
+            held = [(key, list(bufs)) for key, bufs in self._bufs.items()]
+        for index in {key[0] for key, _ in held if key[2]}:
+            torch.cuda.synchronize(index)  # graphs are replayed on other streams than they were captured on
+        for (idx, stream, _), bufs in held:
             if device is not None and idx != device.index:
                 continue
-            st = ctypes.c_int(0)
-            code = L.load().cb_workspace_status(buf.data_ptr(), ctypes.byref(st), stream)
-            if code not in (L.CB_OK, L.CB_ERR_DEVICE_TIMEOUT, L.CB_ERR_DEVICE_INDEX):
-                L.check("cb_workspace_status", code)
-            worst |= st.value
+            for buf in bufs:
+                st = ctypes.c_int(0)
+                code = L.load().cb_workspace_status(buf.data_ptr(), ctypes.byref(st), stream)
+                if code not in (L.CB_OK, L.CB_ERR_DEVICE_TIMEOUT, L.CB_ERR_DEVICE_INDEX):
+                    L.check("cb_workspace_status", code)
+                worst |= st.value
         return worst
 
 
@@ -554,7 +598,7 @@ def _N():
         except ImportError as e:
             raise RuntimeError(f"cb200/_native.so does not load ({e}); build it with cb200.build.build()") from e
         names = ("cb_add_rmsnorm_quant", "cb_quant_act_fp8_block", "cb_fp8_block_gemm", "cb_fp8_block_gemm_dynamic",
-                 "cb_paged_kv_append", "cb_paged_decode_attention", "cb_workspace_bytes")
+                 "cb_paged_kv_append", "cb_paged_decode_attention", "cb_workspace_bytes", "cb_stream_capture_id")
         module.init({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, L.check,
                     lambda nbytes, index: POOL.share(nbytes, torch.device("cuda", index), module))
         _native = module

@@ -35,6 +35,7 @@ struct Api {
   decltype(&cb_paged_kv_append) paged_kv_append;
   decltype(&cb_paged_decode_attention) paged_decode_attention;
   decltype(&cb_workspace_bytes) workspace_bytes;
+  decltype(&cb_stream_capture_id) stream_capture_id;
 } api;
 PyObject* py_check = nullptr;      // _lib.check(name, code): raises
 PyObject* py_workspace = nullptr;  // (bytes, device index): makes the pool register a workspace of that size
@@ -103,11 +104,11 @@ cb_stream_t current_stream(c10::Device d) {
 // ---- workspaces ---------------------------------------------------------------
 struct Key {
   int device;
-  uint64_t stream;
-  bool operator==(const Key& o) const { return device == o.device && stream == o.stream; }
+  uint64_t stream, capture;  // capture: 0 outside a capture
+  bool operator==(const Key& o) const { return device == o.device && stream == o.stream && capture == o.capture; }
 };
 struct KeyHash {
-  size_t operator()(const Key& k) const { return std::hash<uint64_t>()(k.stream * 64 + k.device); }
+  size_t operator()(const Key& k) const { return std::hash<uint64_t>()((k.stream + k.capture * 0x9e3779b97f4a7c15ull) * 64 + k.device); }
 };
 struct Buffer {
   void* p;
@@ -115,9 +116,10 @@ struct Buffer {
 };
 std::unordered_map<Key, Buffer, KeyHash> workspaces;
 
-// The pool's workspace of the device and stream, of at least `need` bytes.
+// The pool's workspace of the device, the stream and the capture that it is in, of at
+// least `need` bytes.
 Buffer workspace(c10::Device d, cb_stream_t stream, size_t need) {
-  const Key key{d.index(), reinterpret_cast<uint64_t>(stream)};
+  const Key key{d.index(), reinterpret_cast<uint64_t>(stream), api.stream_capture_id(stream)};
   auto it = workspaces.find(key);
   if (it == workspaces.end() || it->second.bytes < need) {
     PyObject* r = PyObject_CallFunction(py_workspace, "ni", static_cast<Py_ssize_t>(need), static_cast<int>(d.index()));
@@ -460,6 +462,7 @@ PyObject* init(PyObject* const* a, Py_ssize_t n) {
   CB_ADDR(paged_kv_append);
   CB_ADDR(paged_decode_attention);
   CB_ADDR(workspace_bytes);
+  CB_ADDR(stream_capture_id);
 #undef CB_ADDR
   Py_INCREF(a[1]);
   Py_XDECREF(py_check);
@@ -470,21 +473,35 @@ PyObject* init(PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// (device index, stream, address, bytes)
-PyObject* set_workspace(PyObject* const* a, Py_ssize_t n) {
-  count(n, 4);
+Key key_of(PyObject* const* a) {
   const long device = PyLong_AsLong(a[0]);
-  const uint64_t stream = PyLong_AsUnsignedLongLong(a[1]);
-  void* p = PyLong_AsVoidPtr(a[2]);
-  const size_t bytes = PyLong_AsSize_t(a[3]);
+  const uint64_t stream = PyLong_AsUnsignedLongLong(a[1]), capture = PyLong_AsUnsignedLongLong(a[2]);
   if (PyErr_Occurred()) throw Raised{};
-  workspaces[Key{static_cast<int>(device), stream}] = Buffer{p, bytes};
+  return Key{static_cast<int>(device), stream, capture};
+}
+
+// (device index, stream, capture, address, bytes)
+PyObject* set_workspace(PyObject* const* a, Py_ssize_t n) {
+  count(n, 5);
+  const Key key = key_of(a);
+  void* p = PyLong_AsVoidPtr(a[3]);
+  const size_t bytes = PyLong_AsSize_t(a[4]);
+  if (PyErr_Occurred()) throw Raised{};
+  workspaces[key] = Buffer{p, bytes};
+  Py_RETURN_NONE;
+}
+
+// (device index, stream, capture)
+PyObject* drop_workspace(PyObject* const* a, Py_ssize_t n) {
+  count(n, 3);
+  workspaces.erase(key_of(a));
   Py_RETURN_NONE;
 }
 
 #define CB_ENTRY(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CB_ENTRY(init),
                          CB_ENTRY(set_workspace),
+                         CB_ENTRY(drop_workspace),
                          CB_ENTRY(add_rmsnorm_quant),
                          CB_ENTRY(quant_act_fp8_block),
                          CB_ENTRY(fp8_block_gemm),

@@ -12,7 +12,8 @@
  *     zero-filled once when it is allocated; the kernels leave it zeroed again;
  *   - returns a cb_status code and never aborts the process.
  * A workspace may be used by one stream at a time. Calls that share a workspace
- * on different streams without ordering race.
+ * on different streams without ordering race, and so do graphs whose captured calls
+ * share one: cb_capture_workspace gives each capture its own.
  *
  * Reference interfaces (paths inside the cache-barrier repository) are cited
  * beside each entry point.
@@ -114,6 +115,18 @@ CB_API size_t cb_workspace_bytes(int op, int64_t batch, int64_t M, int64_t N, in
    the cache (and then clears the word and the workspace's arrival counters,
    which a kernel that gave up a wait may leave behind), CB_OK otherwise. */
 CB_API int cb_workspace_status(void* workspace, int* device_status, cb_stream_t stream);
+
+/* Workspaces of captured calls. cb_stream_capture_id: which capture the stream is in, 0
+   for none; never the same for two captures. cb_capture_workspace: during a capture, a
+   zeroed workspace of the current device for calls captured on `stream`. It belongs to
+   the graph: nothing else uses it until the graph and all that was instantiated from it
+   are destroyed and their last execution is over; the library then gives it to a later
+   capture (device memory is allocated here, outside the capture, and by no other entry
+   that takes a workspace). cb_capture_live: 1 as long as such a workspace of that capture
+   belongs to a graph, else 0. */
+CB_API uint64_t cb_stream_capture_id(cb_stream_t stream);
+CB_API int cb_capture_workspace(cb_stream_t stream, size_t bytes, void** workspace);
+CB_API int cb_capture_live(uint64_t capture_id);
 
 /* Failure-detection test hook (no counterpart in the reference). With a
    nonzero limit_ns, every later W8A8 GEMM launch (all W8A8 entry points and
