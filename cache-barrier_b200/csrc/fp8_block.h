@@ -19,6 +19,10 @@ struct BlockGemmArgs {
   void* workspace;
 };
 
+// Bytes that a tile of `width` channels holds of an output row that has `channels` left
+// (up to 2^30: times their size more than an int).
+__host__ __device__ inline int tile_bytes(int channels, int width, int elem) { return (channels < width ? channels : width) * elem; }
+
 // What joining a tile's parts costs, in k-blocks: `join`, and `each` for every `per`
 // parts after the first.
 struct JoinCost {

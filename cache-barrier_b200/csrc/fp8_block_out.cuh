@@ -64,7 +64,7 @@ __device__ __forceinline__ void store_rows(uint8_t* stg, const float (&sum)[C], 
                                            int dtype, int unit, int lane) {
   auto flush = [&](int byte0, int elem) {
     __syncwarp();
-    const int bytes = channels * elem - byte0;
+    const int bytes = tile_bytes(channels, C, elem) - byte0;
     if (unit == 16)
       flush_rows<uint4>(stg, out + byte0, row_bytes, rows, bytes, lane);
     else if (unit == 4)
