@@ -582,9 +582,12 @@ int launch_quant_fp8_block(const void* a, int a_dtype, int64_t batch, int64_t M,
   p.K = static_cast<int>(K);
   p.groups = static_cast<int>((K + kGroup - 1) / kGroup);
   p.total = batch * M * p.groups;
+  // a dimension of one has no stride
+  if (M == 1) a_sm = q_sm = s_sm = 0;
+  if (batch == 1) a_sb = q_sb = s_sb = 0;
   p.a_sb = a_sb, p.a_sm = a_sm, p.q_sb = q_sb, p.q_sm = q_sm, p.s_sb = s_sb, p.s_sm = s_sm;
-  const bool vec = K % 8 == 0 && vec_rows(a, a_sm, 2) && (batch == 1 || a_sb % 8 == 0) &&
-                   (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && q_sm % 8 == 0 && (batch == 1 || q_sb % 8 == 0);
+  const bool vec = K % 8 == 0 && vec_rows(a, a_sm, 2) && a_sb % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 &&
+                   q_sm % 8 == 0 && q_sb % 8 == 0;
   const long long blocks = (p.total + 15) / 16;
   const dim3 grid(static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20))), block(256);
   if (a_dtype == CB_DTYPE_BF16)

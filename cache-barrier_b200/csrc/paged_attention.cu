@@ -959,12 +959,17 @@ extern "C" CB_API int cb_paged_decode_attention(const void* q, int q_dtype, cons
       max_pages > 0x7fffffffLL || max_pages * page_size > 0x7fffff00LL)
     return CB_ERR_TOO_LARGE;
   const int64_t e = fp8 ? 1 : 2;
-  for (int i = 0; i < 12; ++i)
-    if (strides[i] < 0) return CB_ERR_STRIDE;
+  // a dimension of one has no stride: what is given there is not looked at
+  const int64_t size[12] = {B, Hq, B, Hq, B, B, num_pages, page_size, Hkv, num_pages, page_size, Hkv};
+  int64_t st[12];
+  for (int i = 0; i < 12; ++i) {
+    st[i] = size[i] == 1 ? 0 : strides[i];
+    if (st[i] < 0) return CB_ERR_STRIDE;
+  }
   // cache rows are read in 16-byte vectors
   if (!aligned16(k_cache) || !aligned16(v_cache)) return CB_ERR_ALIGNMENT;
   for (int i = 6; i < 12; ++i)
-    if ((strides[i] * e) % 16 != 0) return CB_ERR_ALIGNMENT;
+    if ((st[i] * e) % 16 != 0) return CB_ERR_ALIGNMENT;
   const int G = static_cast<int>(Hq / Hkv);
   const int nt = head_tiles(G, static_cast<int>(D));
   AttnParams p = {};
@@ -974,14 +979,14 @@ extern "C" CB_API int cb_paged_decode_attention(const void* q, int q_dtype, cons
   p.blocks = (G + 8 * nt - 1) / (8 * nt);
   p.num_pages = static_cast<int>(num_pages), p.page = static_cast<int>(page_size);
   p.max_pages = static_cast<int>(max_pages);
-  p.q_vec = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && strides[0] % 4 == 0 && strides[1] % 4 == 0;
+  p.q_vec = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0;
   p.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (page_size == (1LL << s)) p.page_shift = s;
-  p.q_sb = strides[0], p.q_sh = strides[1], p.o_sb = strides[2], p.o_sh = strides[3];
-  p.lse_sb = strides[4], p.table_sb = strides[5];
-  p.k_sp = strides[6] * e, p.k_ss = strides[7] * e, p.k_sh = strides[8] * e;
-  p.v_sp = strides[9] * e, p.v_ss = strides[10] * e, p.v_sh = strides[11] * e;
+  p.q_sb = st[0], p.q_sh = st[1], p.o_sb = st[2], p.o_sh = st[3];
+  p.lse_sb = st[4], p.table_sb = st[5];
+  p.k_sp = st[6] * e, p.k_ss = st[7] * e, p.k_sh = st[8] * e;
+  p.v_sp = st[9] * e, p.v_ss = st[10] * e, p.v_sh = st[11] * e;
   const long long cap = max_pages * page_size;
   const long long most = B * Hkv * p.blocks * ((cap + kTile - 1) / kTile + kItemCost);
   const size_t need = workspace_need(attn_grid_limit(), part_bytes(G, static_cast<int>(D)));

@@ -177,9 +177,13 @@ extern "C" CB_API int cb_paged_kv_append(const void* k, const void* v, int dtype
   const int64_t ce = cache_dtype == CB_DTYPE_E4M3 ? 1 : 2;
   bool vec = D % 8 == 0;
   for (int i = 0; i < 2; ++i) {
-    const int64_t* st = strides + 5 * i;
-    for (int j = 0; j < 5; ++j)
+    // a dimension of one has no stride: what is given there is not looked at
+    const int64_t size[5] = {T, heads, num_pages, page_size, heads};
+    int64_t st[5];
+    for (int j = 0; j < 5; ++j) {
+      st[j] = size[j] == 1 ? 0 : strides[5 * i + j];
       if (st[j] < 0) return CB_ERR_STRIDE;
+    }
     p.src_st[i] = st[0], p.src_sh[i] = st[1];
     p.dst_sp[i] = st[2], p.dst_ss[i] = st[3], p.dst_sh[i] = st[4];
     // vectors of eight elements: 16 bytes in, 8 or 16 bytes out
