@@ -29,7 +29,7 @@ int launch_block_gemm(const BlockGemmArgs& L, cudaStream_t stream) {
   return launch_block_gemm_tc(L, stream);
 }
 
-// Checks the arguments and fills L. A dimension of one has no stride: what
+// Checks the arguments of both entries and fills L. A dimension of one has no stride: what
 // the caller gives there (frameworks give anything) is not looked at.
 int check_block_gemm(BlockGemmArgs& L, const uint8_t* aq, const float* a_scale, const uint8_t* w, const float* w_scale,
                      const void* bias, int bias_dtype, void* out, int out_dtype, int64_t batch, int64_t M, int64_t N, int64_t K,
@@ -91,10 +91,10 @@ extern "C" CB_API int cb_fp8_block_gemm_dynamic(const void* a, int a_dtype, int6
                                                 size_t workspace_bytes, cb_stream_t stream) {
   if (batch < 0 || M < 0 || N < 0 || K < 0) return CB_ERR_INVALID_ARG;
   if (batch == 0 || M == 0 || N == 0) return CB_OK;
-  if (!strides) return CB_ERR_INVALID_ARG;
-  const int rc = cb_quant_act_fp8_block(a, a_dtype, batch, M, K, a_sb, a_sm, q, strides[0], strides[1], scale,
-                                        strides[6], strides[7], stream);
-  if (rc != CB_OK) return rc;
-  return cb_fp8_block_gemm(q, scale, w, w_scale, bias, bias_dtype, out, out_dtype, batch, M, N, K, strides, workspace,
-                           workspace_bytes, stream);
+  BlockGemmArgs L;
+  int rc = check_block_gemm(L, q, scale, w, w_scale, bias, bias_dtype, out, out_dtype, batch, M, N, K, strides, workspace,
+                            workspace_bytes);
+  if (rc != CB_OK) return rc;  // before anything is written
+  rc = cb_quant_act_fp8_block(a, a_dtype, batch, M, K, a_sb, a_sm, q, L.a_sb, L.a_sm, scale, L.as_sb, L.as_sm, stream);
+  return rc != CB_OK ? rc : launch_block_gemm(L, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -1,6 +1,6 @@
 """Dimensions of size one: their stride is not a distance between anything, and frameworks
 give any value there (torch: 1 for a transposed column). Such tensors are taken as what
-they are."""
+they are, and a call that is refused has written nothing."""
 
 import pytest
 import torch
@@ -62,6 +62,12 @@ def test_dynamic_call(cuda_device, M):
         assert torch.equal(ops.fp8_block_gemm_dynamic(column, w, w_s, q=q, s=s), ref)
         assert torch.equal(q.view(torch.uint8), q_ref.view(torch.uint8)) and torch.equal(s, s_ref)
         assert torch.equal(ops.quant_act_fp8_block(column)[0].view(torch.uint8), q_ref.view(torch.uint8))
+    # refused (rows of w off the 16-byte grid): q and s are as they were
+    wide = torch.zeros(256, 520, dtype=torch.uint8, device=d).view(FP8)[:, :512]
+    q, s = torch.full_like(q_ref.view(torch.uint8), 0x33), torch.full_like(s_ref, 7.0)
+    with pytest.raises(ValueError):
+        ops.fp8_block_gemm_dynamic(a, wide, w_s, q=q.view(FP8), s=s)
+    assert bool((q == 0x33).all()) and bool((s == 7.0).all())
 
 
 def _cache(g, pages, page, heads, D, dtype, d):
