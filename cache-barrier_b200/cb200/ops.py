@@ -133,7 +133,10 @@ class WorkspacePool:
         native.set_workspace(device.index, stream, L.load().cb_stream_capture_id(stream), buf.data_ptr(), buf.numel())
 
     def check_status(self, device: torch.device | None = None) -> int:
-        """Synchronising read of the device status word of every buffer on device."""
+        """Synchronising read of the device status word of every buffer on device
+        (``cuda`` without an index: the current device; None: all)."""
+        if device is not None and device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         worst = 0
         with self._lock:
             self._forget_dead()

@@ -138,3 +138,21 @@ def test_outside_a_capture_the_library_refuses():
     assert lib.cb_capture_workspace(None, 256, ctypes.byref(p)) == L.CB_ERR_INVALID_ARG
     assert lib.cb_capture_workspace(None, 0, ctypes.byref(p)) == L.CB_ERR_INVALID_ARG
     assert lib.cb_capture_workspace(None, 256, None) == L.CB_ERR_INVALID_ARG
+
+
+def test_status_of_the_current_device(world, monkeypatch):
+    """A device without an index is the current one, as everywhere in torch: its errors are seen."""
+    lib, _, pool = world
+
+    class Buffer:
+        def __init__(self, address):
+            self.data_ptr = lambda: address
+
+    pool._bufs = {(0, 7, 0): [Buffer(0x100)], (1, 9, 0): [Buffer(0x200)]}
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    lib.words = {0x100: 1, 0x200: 2}
+    assert pool.check_status(torch.device("cuda")) == 2
+    assert pool.check_status(torch.device("cuda", 0)) == 1
+    assert pool.check_status(torch.device("cuda")) == 0
+    lib.words = {0x100: 1, 0x200: 2}
+    assert pool.check_status() == 3
