@@ -15,10 +15,10 @@
 // Three instructions a value; an IEEE division each (about 20) made the kernels that
 // use this issue-bound. The remainder is taken with its sign turned, so that a zero
 // quotient keeps its sign. Steps whose reciprocal or remainder would leave the normal
-// range (below 2^-60, above 2^126, NaN) are divided, and so, unless BOUNDED, are eight
-// values of which one is beyond 512 steps: where q is infinite, q - r y is not a number.
-// BOUNDED says that no value exceeds 512 steps (steps that come from the values' own
-// maximum; an infinity there makes the step infinite).
+// range (below 2^-60, above 2^126, NaN) are divided, and so are eight values of which one
+// may be beyond 512 steps (`bounded` false): where q is infinite, q - r y is not a number.
+// Values whose step comes from their own maximum are bounded (an infinity among them makes
+// the step infinite).
 #pragma once
 
 #include <cstdint>
@@ -27,25 +27,17 @@
 namespace cb {
 
 // int8 rounds half away from zero, e4m3 to nearest even, saturated.
-template <bool INT8, bool BOUNDED = true>
-__device__ __forceinline__ uint64_t quant8(const float (&u)[8], float step) {
+template <bool INT8>
+__device__ __forceinline__ uint64_t quant8(const float (&u)[8], float step, bool bounded = true) {
   float v[8];
-  bool multiply = step >= 8.673617379884035e-19f && step <= 8.507059173023462e+37f;  // 2^-60, 2^126
-  if (multiply) {
+  if (bounded && step >= 8.673617379884035e-19f && step <= 8.507059173023462e+37f) {  // 2^-60, 2^126
     const float y = __fdiv_rn(1.0f, step);
-    float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      v[j] = __fmul_rn(u[j], y);
-      if constexpr (!BOUNDED) top = fmaxf(top, fabsf(v[j]));  // NaN: stays NaN either way
+      const float q = __fmul_rn(u[j], y);
+      v[j] = __fmaf_rn(-__fmaf_rn(q, step, -u[j]), y, q);
     }
-    if constexpr (!BOUNDED) multiply = top < 512.0f;
-    if (multiply) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __fmaf_rn(-__fmaf_rn(v[j], step, -u[j]), y, v[j]);
-    }
-  }
-  if (!multiply) {
+  } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(u[j], step);
   }

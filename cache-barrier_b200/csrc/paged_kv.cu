@@ -50,6 +50,24 @@ __device__ __forceinline__ void put(__nv_fp8_storage_t* o, float v, float scale)
   *o = __nv_cvt_float_to_fp8(__fdiv_rn(v, scale), __NV_SATFINITE, __NV_E4M3);
 }
 
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+
+// Largest magnitude of eight 16-bit values, as pairs (NaN where all of a half are).
+template <typename T2>
+__device__ __forceinline__ float largest8(const T2* w) {
+  const T2 m = __hmax2(__hmax2(__habs2(w[0]), __habs2(w[1])), __hmax2(__habs2(w[2]), __habs2(w[3])));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
 // threadIdx.x walks a token's vectors, threadIdx.y and kUnroll its tokens: the slots and
 // rows of kUnroll tokens are all requested before the first is used, and the divisions
 // (vector to head, slot to page) are per thread or token, not per vector.
@@ -80,6 +98,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
     const T* src = static_cast<const T*>(p.src[which]) + t0 * p.src_st[which] + h * p.src_sh[which] + at;
     C* dst = static_cast<C*>(p.dst[which]) + h * p.dst_sh[which] + at;
     const float scale = p.scale[which] ? __ldg(p.scale[which] + h) : 1.0f;
+    const float most = 512.0f * scale;  // keys are not bounded by their head's scale
     if constexpr (VEC) {
       uint4 raw[kUnroll];
 #pragma unroll
@@ -98,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
           float u[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) u[j] = to_f32(e[j]);
-          const uint64_t q = quant8<false, false>(u, scale);  // keys are not bounded by their scale
+          const uint64_t q = quant8<false>(u, scale, largest8(reinterpret_cast<const typename Pair<T>::type*>(&raw[x])) < most);
           out = *reinterpret_cast<const Out*>(&q);
         } else {
 #pragma unroll
