@@ -666,8 +666,9 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 
     slots: int32 or int64 ``[T]``, token t goes to page ``slots[t] // page_size``,
     slot ``slots[t] % page_size``; a negative slot skips its token. An e4m3 cache
-    stores ``k / k_scale[head]``, saturated. A slot past the cache is skipped and
-    shows in ``device_status``. Two tokens with the same slot leave either of them."""
+    stores ``k / k_scale[head]``, saturated (infinities too; NaN stays NaN). A slot past
+    the cache is skipped and shows in ``device_status``. Where tokens share a slot, it
+    holds an unspecified mixture of their elements."""
     _N().paged_kv_append(k, v, k_cache, v_cache, slots, k_scale, v_scale)
 
 

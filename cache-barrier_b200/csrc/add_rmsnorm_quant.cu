@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormParams p) {
 // Every thread copies into shared memory just what it will read itself (cp.async), so a
 // row needs no barrier but its reduction's. One CTA per row instead leaves HBM idle
 // while the resident CTAs reduce and store (16384 x 8192 with a residual: 199 us; this
-// form 147, the measured copy rate).
+// form 144 to 164, 0.87 to 1.0 of the copy rate, by the device).
 // The weight stays in registers.
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");

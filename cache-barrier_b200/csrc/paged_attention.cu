@@ -6,17 +6,18 @@
 //
 // Bound: HBM on the cache (2 * L * heads * D elements read once; 2G flops per
 // byte of a 16-bit cache) while sequences are long: eight of 65536 tokens over eight
-// heads of 128 take 287 us, 6.5 TB/s in bf16. An e4m3 cache gives a step of 16 tokens
-// half the bytes for the same instructions and latencies: 64 sequences of 4096 tokens
-// 115 us, 4.1 TB/s (bf16 151 us, 6.2 TB/s). Short sequences are bound by an item's chain
-// (page index, keys, scores, values, join): 256 of up to 1000 tokens 44 us.
+// heads of 128 take 286 to 306 us by the device, 6.1 to 6.5 TB/s in bf16. An e4m3 cache
+// gives a step of 16 tokens half the bytes for the same instructions and latencies: 64
+// sequences of 4096 tokens 117 us, 4.0 TB/s (bf16 149 us, 6.3 TB/s). Short sequences are
+// bound by an item's chain (page index, keys, scores, values, join): 256 of up to 1000
+// tokens 45 us.
 //
 // One pass with a running maximum and sum. All (sequence, kv head, head block)
 // items are cut into tiles of kTile tokens, laid end to end, and the tiles are
 // dealt to the CTAs in equal contiguous ranges, so ragged lengths load every SM
 // alike; an item's set-up counts as kItemCost tiles, and an item of at most
 // kWholeTiles stays whole with the CTA that holds its first unit (64 mixed lengths,
-// e4m3: 92 us before these rules and the early requests below, 45 with them). An item
+// e4m3: 92 us before these rules and the early requests below, 46 with them). An item
 // inside one CTA's range is finished there; a cut item's parts (max, sum, unnormalised output per head) go to the workspace
 // and the CTA whose atomic completes the item's count joins them in CTA order: no CTA
 // waits, and the bits do not depend on who joins. Where an item has kPartsApart parts
@@ -24,7 +25,7 @@
 // tokens over one head: 120 us joined by the last CTA, 31 us apart).
 //
 // Giving each short item to one warp alone (four items' chains at once, no barriers)
-// was slower: 52 us against 45 for the 256 sequences, at four times the steps per chain.
+// was slower: 52 us against 44 for the 256 sequences, at four times the steps per chain.
 //
 // A CTA is four warps, and each warp is a worker of its own: it takes 16 of a
 // tile's tokens and keeps its own running maximum, sum and output, so the loop
@@ -248,8 +249,8 @@ struct Shape {
   static constexpr int kVC = kVLane / kVV;
   static constexpr int kKSteps = D / 16;
   // CTAs per SM that the registers are to leave room for. Heads of 128 over e4m3 run four
-  // (180 sequences of 5825 tokens, one query per head: 204 us, with three 219); bf16
-  // needs its registers for 16-byte loads in flight.
+  // (180 sequences of 5825 tokens, one query per head, with one term per probability:
+  // 204 us, with three 219); bf16 needs its registers for 16-byte loads in flight.
   static constexpr int kMinCtas = D == 64 || (FP8 && D == 128 && NT == 1) ? 4 : NT == 1 && (D == 128 || FP8) ? 3 : 2;
   // part of a cut item: max and sum per head, output per head and d
   static constexpr int kPart = kHeads * 2 + kHeads * D;

@@ -440,11 +440,12 @@ CB_API int cb_fp8_block_gemm_dynamic(const void* a, int a_dtype, int64_t a_sb, i
 /* Writes new keys and values [T, heads, D] (f16/bf16) into paged caches of
    num_pages x page_size slots: token t goes to slot slots[t] (int32, or int64 with
    slots_i64), page slot / page_size. cache_dtype: f16, bf16 or e4m3; an e4m3 cache
-   stores row / scale[head], saturated (k_scale, v_scale: [heads] fp32, null = 1).
-   A negative slot skips its token; a slot past the cache is skipped too and sets
-   bit 2 of *status (nullable; a workspace's first word). Two tokens with one slot
-   leave either. strides (elements): {k_t, k_h, kcache_page, kcache_slot,
-   kcache_head} and the same five for v. */
+   stores row / scale[head], saturated, infinities too (k_scale, v_scale: [heads]
+   fp32, null = 1). A negative slot skips its token; a slot past the cache is
+   skipped too and sets bit 2 of *status (nullable; a workspace's first word). A
+   slot that several tokens share holds an unspecified mixture of their elements.
+   strides (elements): {k_t, k_h, kcache_page, kcache_slot, kcache_head} and the
+   same five for v. */
 CB_API int cb_paged_kv_append(const void* k, const void* v, int dtype, void* k_cache, void* v_cache, int cache_dtype,
                               const float* k_scale, const float* v_scale, const void* slots, int slots_i64, int64_t T,
                               int64_t heads, int64_t D, int64_t num_pages, int64_t page_size, const int64_t* strides,
