@@ -120,3 +120,23 @@ def test_infinite_values_stay_infinite(cuda_device, dtype):
     ref = torch.einsum("hgl,lhd->hgd", p, v.double()).reshape(1, 4, 64)
     assert torch.equal(torch.isinf(out), torch.isinf(ref)) and torch.equal(torch.isnan(out), torch.isnan(ref))
     assert torch.equal(out[torch.isinf(ref)], ref[torch.isinf(ref)]) and int(torch.isinf(ref).sum()) == 4
+
+
+@pytest.mark.parametrize("dtype,cache_dtype,top", [(torch.bfloat16, torch.bfloat16, 1e34), (torch.float16, torch.float16, 65504.0),
+                                                   (torch.bfloat16, FP8, 448.0)])
+def test_vanishing_weights_add_nothing(cuda_device, dtype, cache_dtype, top):
+    """The first token holds all the weight and a small value; 20000 others are 2^-200 of it, with large values (whose
+    plain sum fp32 still holds). Many sequences over the same pages, so that each CTA meets thousands of them."""
+    from cb200 import ops
+    L, D, Hkv, B, page = 20000, 64, 8, 64, 64
+    q = torch.zeros(B, Hkv, D, dtype=dtype, device=cuda_device)
+    q[..., 0] = 16.0
+    k = torch.zeros(-(-L // page), page, Hkv, D)
+    k[..., 0] = -70.0
+    k[0, 0, :, 0] = 0.0
+    v = torch.full(k.shape, top)
+    v[0, 0] = 2.0 ** -6
+    table = torch.arange(k.shape[0], dtype=torch.int32, device=cuda_device).expand(B, -1).contiguous()
+    out = ops.paged_decode_attention(q, k.to(cache_dtype).to(cuda_device), v.to(cache_dtype).to(cuda_device), table,
+                                     torch.full((B,), L, dtype=torch.int32, device=cuda_device))
+    assert torch.all(out == 2.0 ** -6), float(out.float().max())
